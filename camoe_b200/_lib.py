@@ -33,6 +33,11 @@ TM_EXPORTS = ("camoe_tm_work_bytes", "camoe_tm_mix_fwd", "camoe_tm_mix_fwd_prev"
               "camoe_tm_prep_bwd", "camoe_tm_post_fwd", "camoe_tm_post_bwd", "camoe_tm_lnsa_fwd",
               "camoe_tm_lnsa_bwd", "camoe_tm_lora_work_bytes", "camoe_tm_lora_wgrad")
 
+# include/camoe_experts.h: the expert layer and the adapters
+EX_EXPORTS = ("camoe_ex_dispatch_work_bytes", "camoe_ex_dispatch", "camoe_ex_combine",
+              "camoe_ex_combine_bwd", "camoe_ex_ffn_fwd", "camoe_ex_ffn_bwd",
+              "camoe_ad_work_bytes", "camoe_ad_linear")
+
 
 class CamoeError(RuntimeError):
     """A non-zero status from the C ABI."""
@@ -101,6 +106,19 @@ def lib() -> ctypes.CDLL:
         getattr(l, n).restype = ci
     l.camoe_tm_lora_work_bytes.restype = sz
     l.camoe_tm_lora_work_bytes.argtypes = [i64] * 3
+    l.camoe_ex_dispatch_work_bytes.restype = sz
+    l.camoe_ex_dispatch_work_bytes.argtypes = [i64] * 3
+    l.camoe_ex_dispatch.argtypes = [vp, ci, vp, ci] + [vp] * 5 + [sz] + [i64] * 4 + [vp]
+    l.camoe_ex_combine.argtypes = [vp, ci] + [vp] * 3 + [i64] * 3 + [vp]
+    l.camoe_ex_combine_bwd.argtypes = [vp, ci] + [vp] * 6 + [i64] * 4 + [vp]
+    l.camoe_ex_ffn_fwd.argtypes = [vp] * 6 + [i64] * 4 + [vp]
+    l.camoe_ex_ffn_bwd.argtypes = [vp] * 10 + [i64] * 4 + [vp]
+    l.camoe_ad_work_bytes.restype = sz
+    l.camoe_ad_work_bytes.argtypes = [i64] * 5
+    l.camoe_ad_linear.argtypes = [vp] * 8 + [sz] + [i64] * 5 + [vp]
+    for n in EX_EXPORTS:
+        if not n.endswith("bytes"):
+            getattr(l, n).restype = ci
     # the wind op's entry points take the ClampW ones' argument types
     l.camoe_wkv7_wind_fwd.restype = ci
     l.camoe_wkv7_wind_fwd.argtypes = l.camoe_wkv7_fwd.argtypes

@@ -1,0 +1,228 @@
+// A projection with the low-rank adapter of each row beside it (declared in
+// include/camoe_experts.h):
+//   y[n] = weight x[n] + scale[a] up[a] (down[a] x[n]),  a = adapter[n]
+//
+// Few rows (a token of each of many requests): two launches.  low[n] = scale[a]
+// down[a] x[n] in fp32, a warp per output; then the projection with the weights
+// streamed once (rows_mma.cuh), to whose sums each output adds its row of up
+// times low, in fp32, before the one rounding.
+//
+// Many rows (prompts): the rows are sorted by adapter, low = scale (xs down^T)
+// is one grouped product (rounded to bf16, the type of the next product's
+// operand), and the projection is a grouped product over the same sorted rows
+// whose sum runs over [x | low] against [weight | up[a]]: the adapter is D more
+// columns of K in the tensor cores, its bytes are read once per row tile, and
+// the result goes to the row that it came from.
+#include "camoe_experts.h"
+#include "rows_mma.cuh"
+#include "tc_launch.cuh"
+
+namespace camoe {
+namespace rows {
+size_t sort_bytes(int64_t N, int64_t k, int64_t E);  // experts_rows.cu
+int sort_rows(const void* x, const int* group, void* xs, int* offsets, int* position, int* source, void* work,
+              int64_t N, int L, int64_t V, cudaStream_t st);
+}  // namespace rows
+
+unsigned int adapter_timeouts() {
+  unsigned int n = 0;
+  if (cudaMemcpyFromSymbol(&n, g_wkv7_timeouts, sizeof(n)) != cudaSuccess) return ~0u;
+  return n;
+}
+
+namespace adapt {
+
+constexpr int kThreads = 256;
+
+// low[n][d] = scale[a] (x[n] . down[a][d]): a warp per (n, d)
+__global__ void __launch_bounds__(kThreads) low_kernel(const bf16* __restrict__ x,
+                                                       const bf16* __restrict__ down,
+                                                       const int* __restrict__ adapter,
+                                                       const float* __restrict__ scale,
+                                                       float* __restrict__ low, int C, int D, int L) {
+  const int n = blockIdx.y, lane = threadIdx.x & 31;
+  const int d = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const int a = adapter[n];
+  if (a < 0 || a >= L || d >= D) return;
+  const uint4* xp = reinterpret_cast<const uint4*>(x + static_cast<int64_t>(n) * C);
+  const bf16* dp = down + (static_cast<int64_t>(a) * D + d) * C;
+  float s = 0.0f;
+  for (int v = lane; v < C / 8; v += 32) {
+    const uint4 p = xp[v], q = thin::ld_once(dp + 8 * v);
+    const __nv_bfloat162* ph = reinterpret_cast<const __nv_bfloat162*>(&p);
+    const __nv_bfloat162* qh = reinterpret_cast<const __nv_bfloat162*>(&q);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = __bfloat1622float2(ph[e]), g = __bfloat1622float2(qh[e]);
+      s = fmaf(f.x, g.x, s);
+      s = fmaf(f.y, g.y, s);
+    }
+  }
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+  if (lane == 0) low[static_cast<int64_t>(n) * D + d] = scale != nullptr ? scale[a] * s : s;
+}
+
+template <int kN>
+__global__ void __launch_bounds__(thin::kThreads) thin_kernel(const bf16* __restrict__ x,
+                                                              const bf16* __restrict__ w,
+                                                              const bf16* __restrict__ up,
+                                                              const int* __restrict__ adapter,
+                                                              const float* __restrict__ low,
+                                                              bf16* __restrict__ y, int64_t N, int C, int M, int D,
+                                                              int L) {
+  __shared__ __align__(16) float red[thin::kWarps * thin::kO * 8 * kN];
+  const int o0 = blockIdx.x * thin::kO, n_o = M - o0 < thin::kO ? M - o0 : thin::kO;
+  const int64_t p = static_cast<int64_t>(blockIdx.y) * 8 * kN;
+  const int n_r = N - p < 8 * kN ? static_cast<int>(N - p) : 8 * kN;
+  thin::block_sums<kN>(w + static_cast<int64_t>(o0) * C, n_o, x + p * C, n_r, C, red);
+  for (int i = threadIdx.x; i < thin::kO * 8 * kN; i += thin::kThreads) {
+    const int o = i % thin::kO, r = i / thin::kO;
+    if (o >= n_o || r >= n_r) continue;
+    float v = thin::total<kN>(red, o, r);
+    const int a = adapter[p + r];
+    if (a >= 0 && a < L) {
+      const uint4* u = reinterpret_cast<const uint4*>(up + (static_cast<int64_t>(a) * M + o0 + o) * D);
+      const float4* l = reinterpret_cast<const float4*>(low + (p + r) * D);
+      float s = 0.0f;
+      for (int d = 0; d < D / 8; ++d) {
+        const uint4 q = u[d];
+        const float4 l0 = l[2 * d], l1 = l[2 * d + 1];
+        const __nv_bfloat162* qh = reinterpret_cast<const __nv_bfloat162*>(&q);
+        const float2 q0 = __bfloat1622float2(qh[0]), q1 = __bfloat1622float2(qh[1]),
+                     q2 = __bfloat1622float2(qh[2]), q3 = __bfloat1622float2(qh[3]);
+        s = fmaf(q0.x, l0.x, s);
+        s = fmaf(q0.y, l0.y, s);
+        s = fmaf(q1.x, l0.z, s);
+        s = fmaf(q1.y, l0.w, s);
+        s = fmaf(q2.x, l1.x, s);
+        s = fmaf(q2.y, l1.y, s);
+        s = fmaf(q3.x, l1.z, s);
+        s = fmaf(q3.y, l1.w, s);
+      }
+      v += s;
+    }
+    y[(p + r) * M + o0 + o] = __float2bfloat16_rn(v);
+  }
+}
+
+// Rows that are streamed rather than sorted: a few, or so few per adapter that
+// row tiles of one adapter each would be mostly empty.
+bool few_rows(int64_t N, int64_t L) { return N <= 256 || N < 16 * L; }
+
+size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+
+struct Layout {  // of the workspace
+  size_t low, xs, offsets, position, source, sort, total;
+};
+Layout layout(int64_t N, int64_t C, int64_t D, int64_t L) {
+  Layout w{};
+  const size_t n = static_cast<size_t>(N);
+  if (few_rows(N, L)) {
+    w.total = up16(n * static_cast<size_t>(D) * sizeof(float));
+    return w;
+  }
+  size_t at = 0;
+  const auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += up16(bytes);
+    return here;
+  };
+  w.low = take(n * static_cast<size_t>(D) * sizeof(bf16));
+  w.xs = take(n * static_cast<size_t>(C) * sizeof(bf16));
+  w.offsets = take(static_cast<size_t>(L + 2) * sizeof(int));
+  w.position = take(n * sizeof(int));
+  w.source = take(n * sizeof(int));
+  w.sort = take(rows::sort_bytes(N, 1, L));
+  w.total = at;
+  return w;
+}
+
+int check(int64_t N, int64_t C, int64_t M, int64_t D, int64_t L) {
+  if (N < 0 || C < 1 || M < 1 || D < 1 || L < 1) return 1;
+  if (C % 8 != 0 || M % 8 != 0 || D % 8 != 0 || D > 256 || L > 1024) return 2;
+  if (N > (1 << 27) || C > (1 << 24) || M > (1 << 24)) return 3;
+  return 0;
+}
+
+template <int kBN>
+int low_product(const bf16* xs, const void* down, const tc::Args& a, int64_t L, cudaStream_t st) {
+  return tc::launch<1, kBN, false, false, false, tc::kScale>({xs, a.K, a.R, 1}, {down, a.K, a.N, L}, {}, {}, a, st);
+}
+
+}  // namespace adapt
+}  // namespace camoe
+
+extern "C" {
+
+size_t camoe_ad_work_bytes(int64_t N, int64_t C, int64_t M, int64_t D, int64_t L) {
+  return camoe::adapt::check(N, C, M, D, L) == 0 ? camoe::adapt::layout(N, C, D, L).total : 0;
+}
+
+int camoe_ad_linear(const void* x, const void* weight, const void* down, const void* up, const int32_t* adapter,
+                    const float* scale, void* y, void* work, size_t work_bytes, int64_t N, int64_t C, int64_t M,
+                    int64_t D, int64_t L, void* stream) {
+  using namespace camoe;
+  using namespace camoe::adapt;
+  if (const int st = check(N, C, M, D, L)) return st;
+  if (N == 0) return 0;
+  for (const void* p : {x, weight, down, up, static_cast<const void*>(adapter), static_cast<const void*>(y),
+                        static_cast<const void*>(work)})
+    if (p == nullptr) return 1;
+  for (const void* p : {x, weight, down, up, static_cast<const void*>(y), static_cast<const void*>(work)})
+    if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0) return 4;
+  const Layout w = layout(N, C, D, L);
+  if (work_bytes < w.total) return 5;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  unsigned char* base = static_cast<unsigned char*>(work);
+  const int c = static_cast<int>(C), m = static_cast<int>(M), d = static_cast<int>(D), l = static_cast<int>(L);
+  const bf16* xb = static_cast<const bf16*>(x);
+  if (few_rows(N, L)) {
+    float* low = static_cast<float*>(work);
+    for (int64_t n0 = 0; n0 < N; n0 += 32768) {  // grid.y holds 65535
+      const int64_t n = N - n0 < 32768 ? N - n0 : 32768;
+      low_kernel<<<dim3((d + 7) / 8, static_cast<unsigned>(n)), kThreads, 0, s>>>(
+          xb + n0 * C, static_cast<const bf16*>(down), adapter + n0, scale, low + n0 * D, c, d, l);
+    }
+    const unsigned gx = static_cast<unsigned>((M + thin::kO - 1) / thin::kO);
+    if (N <= 8)
+      thin_kernel<1><<<dim3(gx, 1), thin::kThreads, 0, s>>>(xb, static_cast<const bf16*>(weight),
+                                                            static_cast<const bf16*>(up), adapter, low,
+                                                            static_cast<bf16*>(y), N, c, m, d, l);
+    else
+      thin_kernel<4><<<dim3(gx, static_cast<unsigned>((N + 31) / 32)), thin::kThreads, 0, s>>>(
+          xb, static_cast<const bf16*>(weight), static_cast<const bf16*>(up), adapter, low,
+          static_cast<bf16*>(y), N, c, m, d, l);
+    return camoe::tm::status(cudaGetLastError());
+  }
+  bf16* low = reinterpret_cast<bf16*>(base + w.low);
+  bf16* xs = reinterpret_cast<bf16*>(base + w.xs);
+  int* offsets = reinterpret_cast<int*>(base + w.offsets);
+  int* source = reinterpret_cast<int*>(base + w.source);
+  if (const int st = rows::sort_rows(x, adapter, xs, offsets, reinterpret_cast<int*>(base + w.position), source,
+                                     base + w.sort, N, l, C / 8, s))
+    return st;
+  tc::Args a{};
+  a.offsets = offsets;
+  a.groups = l;
+  a.R = N;
+  a.N = d;
+  a.K = c;
+  a.out = low;
+  a.scale = scale;
+  const int st = D <= 64 ? low_product<64>(xs, down, a, L, s)
+                         : (D <= 128 ? low_product<128>(xs, down, a, L, s) : low_product<256>(xs, down, a, L, s));
+  if (st != 0) return st;
+  a.groups = l + 1;
+  a.N = m;
+  a.K2 = d;
+  a.groups2 = l;
+  a.b_shared = 1;
+  a.out = static_cast<bf16*>(y);
+  a.scale = nullptr;
+  a.scatter = source;
+  return tc::launch<1, 256, false, false, false, tc::kPlain>({xs, C, N, 1}, {weight, C, M, 1}, {low, D, N, 1},
+                                                             {up, D, M, L}, a, s);
+}
+
+}  // extern "C"

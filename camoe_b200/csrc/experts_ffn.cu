@@ -1,0 +1,212 @@
+// The experts' squared-ReLU products over sorted rows (declared in
+// include/camoe_experts.h): forward in two grouped products, backward in four.
+//
+//   h    = relu(xs w_up^T)^2          rows, K = C, k contiguous in both
+//   ys   = h w_down^T                 rows, K = F
+//   dpre = (dys w_down) 2 sqrt(h)     rows, K = C, w_down read with n contiguous
+//   dxs  = dpre w_up                  rows, K = F, w_up read with n contiguous
+//   dw_up   = dpre^T xs               sums over an expert's rows
+//   dw_down = dys^T h
+//
+// h and dpre are held in bf16, the type of the products' operands.  relu(pre) is
+// not kept: it is sqrt(h), whose rounding error is half of h's.
+#include "camoe_experts.h"
+#include "rows_mma.cuh"
+#include "tc_gemm.cuh"
+#include "tc_launch.cuh"
+
+namespace camoe {
+namespace tm {
+int status(cudaError_t e);  // timemix.cu
+}  // namespace tm
+
+unsigned int ffn_timeouts() {
+  unsigned int n = 0;
+  if (cudaMemcpyFromSymbol(&n, g_wkv7_timeouts, sizeof(n)) != cudaSuccess) return ~0u;
+  return n;
+}
+
+namespace ffn {
+
+// The y-th group that has rows; false where there are fewer.
+__device__ __forceinline__ bool nth_group(const int* offsets, int E, int64_t R, int y, int* g, int64_t* r0,
+                                          int64_t* r1) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int e0 = 0; e0 < E; e0 += 32) {
+    const int e = e0 + lane;
+    int64_t a = 0, b = 0;
+    if (e < E) {
+      a = offsets[e];
+      b = offsets[e + 1];
+      a = a < 0 ? 0 : (a < R ? a : R);
+      b = b < 0 ? 0 : (b < R ? b : R);
+    }
+    unsigned has = __ballot_sync(0xffffffffu, b > a);
+    const int n = __popc(has);
+    if (y < before + n) {
+      for (int i = before; i < y; ++i) has &= has - 1;
+      const int src = __ffs(has) - 1;
+      *g = e0 + src;
+      *r0 = __shfl_sync(0xffffffffu, a, src);
+      *r1 = __shfl_sync(0xffffffffu, b, src);
+      return true;
+    }
+    before += n;
+  }
+  return false;
+}
+
+// out[p][o] = f(sum over k x[p][k] w[e][o][k]) for 16 of the O outputs of the
+// blockIdx.y-th expert that has rows, 8 kN rows at a time.
+template <int kN, bool kRelu2>
+__global__ void __launch_bounds__(thin::kThreads) thin_kernel(const bf16* __restrict__ x,
+                                                              const bf16* __restrict__ w,
+                                                              const int* __restrict__ offsets,
+                                                              bf16* __restrict__ out, int64_t R, int E, int O,
+                                                              int K, int zero_tail) {
+  __shared__ __align__(16) float red[thin::kWarps * thin::kO * 8 * kN];
+  if (zero_tail && blockIdx.y == 0) {
+    const int64_t used = offsets[E] > 0 ? offsets[E] : 0;
+    for (int64_t i = used * O + static_cast<int64_t>(blockIdx.x) * thin::kThreads + threadIdx.x; i < R * O;
+         i += static_cast<int64_t>(gridDim.x) * thin::kThreads)
+      out[i] = __float2bfloat16_rn(0.0f);
+  }
+  int e;
+  int64_t r0, r1;
+  if (!nth_group(offsets, E, R, blockIdx.y, &e, &r0, &r1)) return;
+  const int o0 = blockIdx.x * thin::kO, n_o = O - o0 < thin::kO ? O - o0 : thin::kO;
+  const bf16* we = w + (static_cast<int64_t>(e) * O + o0) * K;
+  for (int64_t p = r0; p < r1; p += 8 * kN) {
+    const int n_r = r1 - p < 8 * kN ? static_cast<int>(r1 - p) : 8 * kN;
+    thin::block_sums<kN>(we, n_o, x + p * K, n_r, K, red);
+    for (int i = threadIdx.x; i < thin::kO * 8 * kN; i += thin::kThreads) {
+      const int o = i % thin::kO, r = i / thin::kO;
+      if (o < n_o && r < n_r) {
+        float v = thin::total<kN>(red, o, r);
+        if (kRelu2) v = v < 0.0f ? 0.0f : v * v;
+        out[(p + r) * O + o0 + o] = __float2bfloat16_rn(v);
+      }
+    }
+    __syncthreads();  // red is written again
+  }
+}
+
+// Few rows per expert: the weights' bytes decide, and the streaming kernel reads
+// them at HBM rate; with more rows than that the tensor memory kernel is faster.
+bool few_rows(int64_t R, int64_t E) { return R <= 16 * E && R <= 512; }
+
+template <bool kRelu2>
+int thin_product(const bf16* x, const bf16* w, const int* offsets, bf16* out, int64_t R, int64_t E, int64_t O,
+                 int64_t K, bool zero_tail, cudaStream_t st) {
+  const dim3 g(static_cast<unsigned>((O + thin::kO - 1) / thin::kO), static_cast<unsigned>(E < R ? E : R));
+  const int e = static_cast<int>(E), o = static_cast<int>(O), k = static_cast<int>(K);
+  if (R <= 2 * E)
+    thin_kernel<1, kRelu2><<<g, thin::kThreads, 0, st>>>(x, w, offsets, out, R, e, o, k, zero_tail);
+  else
+    thin_kernel<4, kRelu2><<<g, thin::kThreads, 0, st>>>(x, w, offsets, out, R, e, o, k, zero_tail);
+  return camoe::tm::status(cudaGetLastError());
+}
+
+tc::Args args(const int* offsets, int64_t E, int64_t R, int64_t N, int64_t K, void* out) {
+  tc::Args a{};
+  a.offsets = offsets;
+  a.groups = static_cast<int>(E);
+  a.R = R;
+  a.N = static_cast<int>(N);
+  a.K = static_cast<int>(K);
+  a.out = static_cast<bf16*>(out);
+  return a;
+}
+
+// rows x grouped weights; w is [E][N][K], or [E][K][N] where kBMN
+template <bool kBMN, int kEpi>
+int rows_product(const void* x, const void* w, const tc::Args& a, int64_t E, cudaStream_t st) {
+  return tc::launch<1, 256, false, kBMN, false, kEpi>(
+      {x, a.K, a.R, 1}, kBMN ? tc::Matrix{w, a.N, a.K, E} : tc::Matrix{w, a.K, a.N, E}, {}, {}, a, st);
+}
+
+int check(const int* offsets, int64_t R, int64_t E, int64_t C, int64_t F) {
+  if (R < 0 || E < 1 || C < 1 || F < 1) return 1;
+  if (E > 1024 || C % 8 != 0 || F % 8 != 0) return 2;
+  if (R > 0x7fffffffLL || C > (1 << 24) || F > (1 << 24)) return 3;
+  return offsets == nullptr ? 1 : 0;
+}
+
+template <typename... Ptr>
+bool aligned(Ptr... p) {
+  uintptr_t all = 0;
+  ((all |= reinterpret_cast<uintptr_t>(p)), ...);
+  return (all & 15u) == 0;
+}
+
+}  // namespace ffn
+}  // namespace camoe
+
+extern "C" {
+
+int camoe_ex_ffn_fwd(const void* xs, const void* w_up, const void* w_down, const int32_t* offsets, void* h,
+                     void* ys, int64_t R, int64_t E, int64_t C, int64_t F, void* stream) {
+  using namespace camoe;
+  using namespace camoe::ffn;
+  if (const int st = check(offsets, R, E, C, F)) return st;
+  if (R == 0) return 0;
+  if (xs == nullptr || w_up == nullptr || w_down == nullptr || h == nullptr || ys == nullptr) return 1;
+  if (!aligned(xs, w_up, w_down, h, ys)) return 4;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (few_rows(R, E)) {
+    const int st = thin_product<true>(static_cast<const bf16*>(xs), static_cast<const bf16*>(w_up), offsets,
+                                      static_cast<bf16*>(h), R, E, F, C, false, s);
+    if (st != 0) return st;
+    return thin_product<false>(static_cast<const bf16*>(h), static_cast<const bf16*>(w_down), offsets,
+                               static_cast<bf16*>(ys), R, E, C, F, true, s);
+  }
+  if (const int st = rows_product<false, tc::kRelu2>(xs, w_up, args(offsets, E, R, F, C, h), E, s)) return st;
+  tc::Args down = args(offsets, E, R, C, F, ys);
+  down.zero_tail = 1;
+  return rows_product<false, tc::kPlain>(h, w_down, down, E, s);
+}
+
+int camoe_ex_ffn_bwd(const void* dys, const void* xs, const void* w_up, const void* w_down,
+                     const int32_t* offsets, const void* h, void* dpre, void* dxs, void* dw_up, void* dw_down,
+                     int64_t R, int64_t E, int64_t C, int64_t F, void* stream) {
+  using namespace camoe;
+  using namespace camoe::ffn;
+  if (const int st = check(offsets, R, E, C, F)) return st;
+  if (!aligned(dys, xs, w_up, w_down, h, dpre, dxs, dw_up, dw_down)) return 4;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (R == 0) {
+    const size_t bytes = static_cast<size_t>(E * C * F) * sizeof(bf16);
+    if (dw_up != nullptr)
+      if (const int st = camoe::tm::status(cudaMemsetAsync(dw_up, 0, bytes, s))) return st;
+    return dw_down != nullptr ? camoe::tm::status(cudaMemsetAsync(dw_down, 0, bytes, s)) : 0;
+  }
+  if (dys == nullptr || h == nullptr) return 1;
+  if (dxs != nullptr || dw_up != nullptr) {
+    if (w_down == nullptr || dpre == nullptr) return 1;
+    tc::Args a = args(offsets, E, R, F, C, dpre);
+    a.aux = static_cast<const bf16*>(h);
+    if (const int st = rows_product<true, tc::kDRelu2>(dys, w_down, a, E, s)) return st;
+  }
+  if (dxs != nullptr) {
+    if (w_up == nullptr) return 1;
+    tc::Args a = args(offsets, E, R, C, F, dxs);
+    a.zero_tail = 1;
+    if (const int st = rows_product<true, tc::kPlain>(dpre, w_up, a, E, s)) return st;
+  }
+  if (dw_up != nullptr) {
+    if (xs == nullptr) return 1;
+    tc::Args a = args(offsets, E, R, C, 0, dw_up);
+    a.M = static_cast<int>(F);
+    if (const int st = tc::launch<1, 256, true, true, true, tc::kPlain>({dpre, F, R, 1}, {xs, C, R, 1}, {}, {}, a, s))
+      return st;
+  }
+  if (dw_down != nullptr) {
+    tc::Args a = args(offsets, E, R, F, 0, dw_down);
+    a.M = static_cast<int>(C);
+    return tc::launch<1, 256, true, true, true, tc::kPlain>({dys, C, R, 1}, {h, F, R, 1}, {}, {}, a, s);
+  }
+  return 0;
+}
+
+}  // extern "C"

@@ -1,0 +1,534 @@
+// Tokens sorted by expert and back (declared in include/camoe_experts.h).
+//
+// The sort is a counting sort that keeps the slots' order: the row of slot s is
+//   #{s' : e(s') < e(s)} + #{s' < s : e(s') = e(s)}
+// with an unused slot counted as expert E, so every slot has exactly one row and
+// the rows behind offsets[E] are those of the unused slots (which get zeros).
+// Counts are integers and nothing depends on the order in which blocks run.
+//
+// Up to kSmallSlots slots one launch does it all: each token's block counts its
+// own slots' rows by reading the whole index once (a warp per slot) and copies
+// its row.  Above that: counts per chunk of 1024 slots, one scan over (expert,
+// chunk), the rows of each chunk's slots, and the copy.
+//
+// The copies are bound by HBM: a thread holds 16 bytes of a row (or one element
+// where the width or an address is no multiple of 16 bytes), a token's row is
+// read once and written k times.
+#include "camoe_experts.h"
+#include "wkv7_common.cuh"
+
+namespace camoe {
+namespace tm {
+int status(cudaError_t e);  // timemix.cu
+}  // namespace tm
+
+namespace rows {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kSmallSlots = 2048;
+constexpr int kChunkSlots = 1024;
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxSlots = 64;  // per token
+constexpr unsigned kFull = 0xffffffffu;
+
+// the expert of slot s, E for an unused one
+template <typename I>
+__device__ __forceinline__ int bin_of(const I* index, int64_t s, int E) {
+  const I e = index[s];
+  return e >= 0 && e < static_cast<I>(E) ? static_cast<int>(e) : E;
+}
+
+// exclusive scan of v over the block (kThreads threads); total in *sum
+__device__ __forceinline__ int block_scan(int v, int* sum) {
+  __shared__ int part[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(kFull, x, d);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();  // part may still be read from an earlier call
+  if (lane == 31) part[warp] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    before += w < warp ? part[w] : 0;
+    all += part[w];
+  }
+  *sum = all;
+  return before + x - v;
+}
+
+// ---- a row in pieces of type P (uint4: 16 bytes; otherwise one element)
+
+template <typename T, typename P>
+struct Piece {
+  static constexpr int n = sizeof(P) / sizeof(T);
+};
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(bf16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ bf16 from_f<bf16>(float x) { return __float2bfloat16_rn(x); }
+
+template <typename T, typename P>
+__device__ __forceinline__ void widen(const P& p, float (&f)[Piece<T, P>::n]) {
+  const T* t = reinterpret_cast<const T*>(&p);
+#pragma unroll
+  for (int i = 0; i < Piece<T, P>::n; ++i) f[i] = to_f(t[i]);
+}
+template <typename T, typename P>
+__device__ __forceinline__ P narrow(const float (&f)[Piece<T, P>::n]) {
+  P p;
+  T* t = reinterpret_cast<T*>(&p);
+#pragma unroll
+  for (int i = 0; i < Piece<T, P>::n; ++i) t[i] = from_f<T>(f[i]);
+  return p;
+}
+template <typename P>
+__device__ __forceinline__ P zero_piece() {
+  P p;
+  memset(&p, 0, sizeof(P));
+  return p;
+}
+
+// ---- sort
+
+// One block per token, and one more for the offsets.
+// kKeep: the slots outside [0, E) are kept, as one more group behind the others
+template <typename I, typename P, bool kKeep>
+__global__ void __launch_bounds__(kThreads) small_kernel(const P* __restrict__ x,
+                                                         const I* __restrict__ index,
+                                                         P* __restrict__ xs, int* __restrict__ offsets,
+                                                         int* __restrict__ position,
+                                                         int* __restrict__ source, int N, int k, int E,
+                                                         int64_t V) {
+  const int S = N * k, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (blockIdx.x == static_cast<unsigned>(N)) {
+    __shared__ int count[kMaxExperts + 1];
+    for (int e = threadIdx.x; e <= E; e += kThreads) count[e] = 0;
+    __syncthreads();
+    for (int s = threadIdx.x; s < S; s += kThreads) atomicAdd(&count[bin_of(index, s, E)], 1);
+    __syncthreads();
+    const int per = (E + kThreads) / kThreads;  // ceil((E + 1) / kThreads)
+    const int first = threadIdx.x * per;
+    int mine = 0, all;
+    for (int e = first; e < first + per && e <= E; ++e) mine += count[e];
+    int at = block_scan(mine, &all);
+    for (int e = first; e < first + per && e <= E; ++e) {
+      offsets[e] = at;
+      at += count[e];
+    }
+    if (kKeep && threadIdx.x == 0) offsets[E + 1] = S;
+    return;
+  }
+  __shared__ int row[kMaxSlots];
+  const int n = blockIdx.x;
+  for (int j = warp; j < k; j += kWarps) {
+    const int s = n * k + j, b = bin_of(index, s, E);
+    int before = 0;
+    for (int i = lane; i < S; i += 32) {
+      const int o = bin_of(index, i, E);
+      before += o < b || (o == b && i < s);
+    }
+    before = __reduce_add_sync(kFull, before);
+    if (lane == 0) {
+      const bool used = kKeep || b < E;
+      row[j] = used ? before : -1 - before;
+      position[s] = used ? before : -1;
+      source[before] = used ? s : -1;
+    }
+  }
+  if (xs == nullptr) return;
+  __syncthreads();
+  for (int64_t v = threadIdx.x; v < V; v += kThreads) {
+    const P p = x[n * V + v];
+    for (int j = 0; j < k; ++j) {
+      const int r = row[j];
+      if (r >= 0)
+        xs[r * V + v] = p;
+      else
+        xs[(-1 - r) * V + v] = zero_piece<P>();
+    }
+  }
+}
+
+// slots of each expert in each chunk: counts[e * chunks + c]
+template <typename I>
+__global__ void __launch_bounds__(kThreads) count_kernel(const I* __restrict__ index,
+                                                         int* __restrict__ counts, int64_t S, int E) {
+  __shared__ int count[kMaxExperts + 1];
+  for (int e = threadIdx.x; e <= E; e += kThreads) count[e] = 0;
+  __syncthreads();
+  const int64_t s0 = static_cast<int64_t>(blockIdx.x) * kChunkSlots;
+#pragma unroll
+  for (int i = 0; i < kChunkSlots / kThreads; ++i) {
+    const int64_t s = s0 + i * kThreads + threadIdx.x;
+    if (s < S) atomicAdd(&count[bin_of(index, s, E)], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e <= E; e += kThreads)
+    counts[static_cast<int64_t>(e) * gridDim.x + blockIdx.x] = count[e];
+}
+
+// counts -> first row of each (expert, chunk), in place; offsets
+template <bool kKeep>
+__global__ void __launch_bounds__(kThreads) scan_kernel(int* __restrict__ counts,
+                                                        int* __restrict__ offsets, int64_t chunks,
+                                                        int64_t S, int E) {
+  constexpr int kPer = 8;
+  if (kKeep && threadIdx.x == 0) offsets[E + 1] = static_cast<int>(S);
+  const int64_t total = (E + 1) * chunks;
+  int carry = 0;
+  for (int64_t i0 = 0; i0 < total; i0 += kThreads * kPer) {
+    const int64_t first = i0 + threadIdx.x * kPer;
+    int c[kPer], mine = 0, all;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      c[i] = first + i < total ? counts[first + i] : 0;
+      mine += c[i];
+    }
+    int at = carry + block_scan(mine, &all);
+    carry += all;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (first + i < total) {
+        counts[first + i] = at;
+        if ((first + i) % chunks == 0) offsets[(first + i) / chunks] = at;
+      }
+      at += c[i];
+    }
+  }
+}
+
+// the row of each slot of a chunk; row[s] = position, or -1 - row of an unused slot
+template <typename I, bool kKeep>
+__global__ void __launch_bounds__(kThreads) place_kernel(const I* __restrict__ index,
+                                                         const int* __restrict__ first,
+                                                         int* __restrict__ position,
+                                                         int* __restrict__ source, int64_t S, int E) {
+  constexpr int kSteps = kChunkSlots / kThreads;
+  extern __shared__ int seen[];  // [kWarps][E + 1]: slots of each expert in a warp's share
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i = threadIdx.x; i < kWarps * (E + 1); i += kThreads) seen[i] = 0;
+  __syncthreads();
+  int* mine = seen + warp * (E + 1);
+  const int64_t s0 = static_cast<int64_t>(blockIdx.x) * kChunkSlots + warp * (kSteps * 32) + lane;
+  int bin[kSteps], rank[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int64_t s = s0 + 32 * i;
+    bin[i] = s < S ? bin_of(index, s, E) : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const unsigned same = __match_any_sync(kFull, bin[i]);
+    const int before = __popc(same & ((1u << lane) - 1u));
+    const int old = bin[i] >= 0 ? mine[bin[i]] : 0;
+    rank[i] = old + before;
+    __syncwarp();
+    if (before == 0 && bin[i] >= 0) mine[bin[i]] = old + __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e <= E; e += kThreads) {
+    int at = first[static_cast<int64_t>(e) * gridDim.x + blockIdx.x];
+    for (int w = 0; w < kWarps; ++w) {
+      const int c = seen[w * (E + 1) + e];
+      seen[w * (E + 1) + e] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int64_t s = s0 + 32 * i;
+    if (bin[i] < 0) continue;
+    const int r = mine[bin[i]] + rank[i];
+    const bool used = kKeep || bin[i] < E;
+    position[s] = used ? r : -1;
+    source[r] = used ? static_cast<int>(s) : -1;
+  }
+}
+
+// ---- copies: blockDim.x threads along a row, blockDim.y tokens
+
+template <typename P>
+__global__ void __launch_bounds__(kThreads) copy_kernel(const P* __restrict__ x,
+                                                        const int* __restrict__ position,
+                                                        P* __restrict__ xs, int64_t N, int k, int64_t V) {
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if (n >= N) return;
+  for (int64_t v = threadIdx.x; v < V; v += blockDim.x) {
+    const P p = x[n * V + v];
+    for (int j = 0; j < k; ++j) {
+      const int r = position[n * k + j];
+      if (r >= 0) xs[r * V + v] = p;  // below N k: the sort's own
+    }
+  }
+}
+
+// zeros in the rows behind offsets[E]
+template <typename P>
+__global__ void __launch_bounds__(kThreads) tail_kernel(const int* __restrict__ offsets, int E,
+                                                        P* __restrict__ xs, int64_t R, int64_t V) {
+  const int64_t end = R * V;
+  const int64_t used = offsets[E] > 0 ? offsets[E] : 0;
+  for (int64_t i = used * V + static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < end;
+       i += static_cast<int64_t>(gridDim.x) * kThreads)
+    xs[i] = zero_piece<P>();
+}
+
+template <typename T, typename P, bool kWeighted>
+__global__ void __launch_bounds__(kThreads) combine_kernel(const P* __restrict__ rows,
+                                                           const float* __restrict__ weight,
+                                                           const int* __restrict__ position,
+                                                           P* __restrict__ out, int64_t N, int k,
+                                                           int64_t V) {
+  constexpr int n_el = Piece<T, P>::n;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if (n >= N) return;
+  for (int64_t v = threadIdx.x; v < V; v += blockDim.x) {
+    float acc[n_el];
+#pragma unroll
+    for (int i = 0; i < n_el; ++i) acc[i] = 0.0f;
+    for (int j = 0; j < k; ++j) {
+      const int64_t r = position[n * k + j];
+      if (r < 0 || r >= N * k) continue;
+      float f[n_el];
+      widen<T, P>(rows[r * V + v], f);
+      const float w = kWeighted ? weight[n * k + j] : 1.0f;
+#pragma unroll
+      for (int i = 0; i < n_el; ++i) acc[i] = kWeighted ? fmaf(w, f[i], acc[i]) : acc[i] + f[i];
+    }
+    out[n * V + v] = narrow<T, P>(acc);
+  }
+}
+
+// a warp per token: its row of dout is held while its slots' rows are read and written
+template <typename T, typename P>
+__global__ void __launch_bounds__(kThreads) combine_bwd_kernel(
+    const P* __restrict__ dout, const P* __restrict__ ys, const float* __restrict__ weight,
+    const int* __restrict__ position, P* __restrict__ dys, float* __restrict__ dweight, int64_t N,
+    int k, int64_t V) {
+  constexpr int n_el = Piece<T, P>::n, kGroup = 4;
+  const int lane = threadIdx.x & 31;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  if (n >= N) return;
+  for (int j0 = 0; j0 < k; j0 += kGroup) {
+    int64_t r[kGroup];
+    float w[kGroup], dot[kGroup];
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j) {
+      r[j] = j0 + j < k ? position[n * k + j0 + j] : -1;
+      if (r[j] >= N * k) r[j] = -1;
+      w[j] = r[j] >= 0 ? weight[n * k + j0 + j] : 0.0f;
+      dot[j] = 0.0f;
+    }
+    for (int64_t v = lane; v < V; v += 32) {
+      float d[n_el];
+      widen<T, P>(dout[n * V + v], d);
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j) {
+        if (r[j] < 0) continue;
+        if (dweight != nullptr) {
+          float f[n_el];
+          widen<T, P>(ys[r[j] * V + v], f);
+#pragma unroll
+          for (int i = 0; i < n_el; ++i) dot[j] = fmaf(d[i], f[i], dot[j]);
+        }
+        if (dys != nullptr) {
+          float g[n_el];
+#pragma unroll
+          for (int i = 0; i < n_el; ++i) g[i] = w[j] * d[i];
+          dys[r[j] * V + v] = narrow<T, P>(g);
+        }
+      }
+    }
+    if (dweight != nullptr) {
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j) {
+#pragma unroll
+        for (int m = 16; m > 0; m >>= 1) dot[j] += __shfl_xor_sync(kFull, dot[j], m);
+        if (lane == 0 && j0 + j < k) dweight[n * k + j0 + j] = r[j] >= 0 ? dot[j] : 0.0f;
+      }
+    }
+  }
+}
+
+// threads along a row of V pieces: a power of two from 32 to kThreads
+inline dim3 row_block(int64_t V) {
+  int tx = 32;
+  while (tx < kThreads && tx < V) tx *= 2;
+  return dim3(tx, kThreads / tx);
+}
+inline int64_t blocks(int64_t N, const dim3& b) { return (N + b.y - 1) / b.y; }
+
+inline int64_t chunks_of(int64_t S) { return (S + kChunkSlots - 1) / kChunkSlots; }
+
+// C elements of 2 or 4 bytes as 16-byte pieces: 0 where that cannot be
+template <typename... Ptr>
+int64_t pieces(int64_t C, int size, Ptr... p) {
+  uintptr_t all = 0;
+  ((all |= reinterpret_cast<uintptr_t>(p)), ...);
+  return (C * size) % 16 == 0 && (all & 15u) == 0 ? C * size / 16 : 0;
+}
+
+int check(int64_t N, int64_t k, int64_t E, int64_t C, int dtype) {
+  if (dtype != 0 && dtype != 1) return 2;
+  if (N < 0 || k < 1 || E < 1 || C < 0) return 1;
+  if (k > kMaxSlots || E > kMaxExperts) return 2;
+  if (N > 0x7fffffffLL / k || C > 0x7fffffffLL) return 3;
+  return 0;
+}
+
+template <typename I, typename P, bool kKeep>
+int sort(const P* x, const I* index, P* xs, int* offsets, int* position, int* source, int* work,
+         int64_t N, int k, int E, int64_t V, cudaStream_t st) {
+  const int64_t S = N * k;
+  if (S <= kSmallSlots) {
+    small_kernel<I, P, kKeep><<<static_cast<unsigned>(N + 1), kThreads, 0, st>>>(
+        x, index, xs, offsets, position, source, static_cast<int>(N), k, E, V);
+    return camoe::tm::status(cudaGetLastError());
+  }
+  const int64_t chunks = chunks_of(S);
+  const unsigned g = static_cast<unsigned>(chunks);
+  count_kernel<I><<<g, kThreads, 0, st>>>(index, work, S, E);
+  scan_kernel<kKeep><<<1, kThreads, 0, st>>>(work, offsets, chunks, S, E);
+  place_kernel<I, kKeep><<<g, kThreads, kWarps * (E + 1) * sizeof(int), st>>>(index, work, position,
+                                                                             source, S, E);
+  if (xs != nullptr && V > 0) {
+    const dim3 b = row_block(V);
+    copy_kernel<P><<<static_cast<unsigned>(blocks(N, b)), b, 0, st>>>(x, position, xs, N, k, V);
+    if (!kKeep) tail_kernel<P><<<148, kThreads, 0, st>>>(offsets, E, xs, S, V);
+  }
+  return camoe::tm::status(cudaGetLastError());
+}
+
+template <typename P>
+int sort_index(const void* x, const void* index, int index_bytes, void* xs, int* offsets, int* position,
+               int* source, int* work, int64_t N, int k, int E, int64_t V, cudaStream_t st) {
+  const P* xp = static_cast<const P*>(x);
+  P* xsp = static_cast<P*>(xs);
+  return index_bytes == 4
+             ? sort<int32_t, P, false>(xp, static_cast<const int32_t*>(index), xsp, offsets, position,
+                                       source, work, N, k, E, V, st)
+             : sort<int64_t, P, false>(xp, static_cast<const int64_t*>(index), xsp, offsets, position,
+                                       source, work, N, k, E, V, st);
+}
+
+size_t sort_bytes(int64_t N, int64_t k, int64_t E) {
+  if (N * k <= kSmallSlots) return 0;
+  return static_cast<size_t>(chunks_of(N * k)) * static_cast<size_t>(E + 1) * sizeof(int);
+}
+
+// For the adapters (adapters.cu): rows of 16-byte pieces by their group, the rows of no group behind
+// the others; offsets has L + 2 entries, row r of xs is row source[r] of x.
+int sort_rows(const void* x, const int* group, void* xs, int* offsets, int* position, int* source,
+              void* work, int64_t N, int L, int64_t V, cudaStream_t st) {
+  return sort<int32_t, uint4, true>(static_cast<const uint4*>(x), group, static_cast<uint4*>(xs), offsets,
+                                    position, source, static_cast<int*>(work), N, 1, L, V, st);
+}
+
+template <typename T, typename P>
+int combine(const void* in, const float* weight, const int* position, void* out, int64_t N, int k,
+            int64_t V, cudaStream_t st) {
+  const dim3 b = row_block(V);
+  const unsigned g = static_cast<unsigned>(blocks(N, b));
+  if (weight != nullptr)
+    combine_kernel<T, P, true><<<g, b, 0, st>>>(static_cast<const P*>(in), weight, position,
+                                                static_cast<P*>(out), N, k, V);
+  else
+    combine_kernel<T, P, false><<<g, b, 0, st>>>(static_cast<const P*>(in), weight, position,
+                                                 static_cast<P*>(out), N, k, V);
+  return camoe::tm::status(cudaGetLastError());
+}
+
+template <typename T, typename P>
+int combine_bwd(const void* dout, const void* ys, const float* weight, const int* offsets,
+                const int* position, void* dys, float* dweight, int64_t N, int k, int E, int64_t V,
+                cudaStream_t st) {
+  combine_bwd_kernel<T, P><<<static_cast<unsigned>((N + kWarps - 1) / kWarps), kThreads, 0, st>>>(
+      static_cast<const P*>(dout), static_cast<const P*>(ys), weight, position, static_cast<P*>(dys),
+      dweight, N, k, V);
+  if (dys != nullptr && V > 0)
+    tail_kernel<P><<<148, kThreads, 0, st>>>(offsets, E, static_cast<P*>(dys), N * k, V);
+  return camoe::tm::status(cudaGetLastError());
+}
+
+}  // namespace rows
+}  // namespace camoe
+
+extern "C" {
+
+size_t camoe_ex_dispatch_work_bytes(int64_t N, int64_t k, int64_t E) {
+  using namespace camoe::rows;
+  return check(N, k, E, 1, 0) == 0 ? sort_bytes(N, k, E) : 0;
+}
+
+int camoe_ex_dispatch(const void* x, int dtype, const void* index, int index_bytes, void* xs,
+                      int32_t* offsets, int32_t* position, int32_t* source, void* work,
+                      size_t work_bytes, int64_t N, int64_t k, int64_t E, int64_t C, void* stream) {
+  using namespace camoe::rows;
+  if (const int st = check(N, k, E, C, dtype)) return st;
+  if (index_bytes != 4 && index_bytes != 8) return 2;
+  if (offsets == nullptr) return 1;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (N == 0)
+    return camoe::tm::status(cudaMemsetAsync(offsets, 0, static_cast<size_t>(E + 1) * sizeof(int), s));
+  if (index == nullptr || position == nullptr || source == nullptr || (xs != nullptr && x == nullptr)) return 1;
+  const size_t need = camoe_ex_dispatch_work_bytes(N, k, E);
+  if (need > 0 && work == nullptr) return 1;
+  if (work_bytes < need) return 5;
+  int* w = static_cast<int*>(work);
+  const int kk = static_cast<int>(k), e = static_cast<int>(E);
+  const int64_t V = pieces(C, dtype == 0 ? 2 : 4, x, xs);
+  if (V > 0) return sort_index<uint4>(x, index, index_bytes, xs, offsets, position, source, w, N, kk, e, V, s);
+  if (dtype == 0)
+    return sort_index<uint16_t>(x, index, index_bytes, xs, offsets, position, source, w, N, kk, e, C, s);
+  return sort_index<uint32_t>(x, index, index_bytes, xs, offsets, position, source, w, N, kk, e, C, s);
+}
+
+int camoe_ex_combine(const void* in, int dtype, const float* weight, const int32_t* position, void* out,
+                     int64_t N, int64_t k, int64_t C, void* stream) {
+  using namespace camoe;
+  using namespace camoe::rows;
+  if (const int st = check(N, k, 1, C, dtype)) return st;
+  if (N == 0 || C == 0) return 0;
+  if (in == nullptr || position == nullptr || out == nullptr) return 1;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int kk = static_cast<int>(k);
+  const int64_t V = pieces(C, dtype == 0 ? 2 : 4, in, out);
+  if (dtype == 0)
+    return V > 0 ? combine<bf16, uint4>(in, weight, position, out, N, kk, V, s)
+                 : combine<bf16, bf16>(in, weight, position, out, N, kk, C, s);
+  return V > 0 ? combine<float, uint4>(in, weight, position, out, N, kk, V, s)
+               : combine<float, float>(in, weight, position, out, N, kk, C, s);
+}
+
+int camoe_ex_combine_bwd(const void* dout, int dtype, const void* ys, const float* weight,
+                         const int32_t* offsets, const int32_t* position, void* dys, float* dweight,
+                         int64_t N, int64_t k, int64_t E, int64_t C, void* stream) {
+  using namespace camoe;
+  using namespace camoe::rows;
+  if (const int st = check(N, k, E, C, dtype)) return st;
+  if (N == 0 || (dys == nullptr && dweight == nullptr)) return 0;
+  if (position == nullptr || weight == nullptr || (dys != nullptr && offsets == nullptr)) return 1;
+  if (C > 0 && (dout == nullptr || (dweight != nullptr && ys == nullptr))) return 1;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int kk = static_cast<int>(k), e = static_cast<int>(E);
+  const int64_t V = pieces(C, dtype == 0 ? 2 : 4, dout, ys, dys);
+  if (dtype == 0)
+    return V > 0 ? combine_bwd<bf16, uint4>(dout, ys, weight, offsets, position, dys, dweight, N, kk, e, V, s)
+                 : combine_bwd<bf16, bf16>(dout, ys, weight, offsets, position, dys, dweight, N, kk, e, C, s);
+  return V > 0 ? combine_bwd<float, uint4>(dout, ys, weight, offsets, position, dys, dweight, N, kk, e, V, s)
+               : combine_bwd<float, float>(dout, ys, weight, offsets, position, dys, dweight, N, kk, e, C, s);
+}
+
+}  // extern "C"

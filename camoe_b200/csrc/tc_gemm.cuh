@@ -1,0 +1,544 @@
+// Products of grouped rows on the 5th-generation tensor cores (tcgen05): one
+// kernel for the experts' six products and the adapters' two.
+//
+// Rows: for the rows p of group g (p in [offsets[g], offsets[g + 1]))
+//     out[p][n] = sum over k of A[p][k] B_g[n][k]  (+ a second pair A2, B2_g)
+//   A's rows have k contiguous; B_g is stored [N][K] (k contiguous) or [K][N]
+//   (n contiguous), which is a bit of the instruction descriptor.
+// Weight gradients: out_g[m][n] = sum over the rows p of g of A[p][m] B[p][n],
+//   both stored with m or n contiguous.
+//
+// One CTA (or a pair of CTAs on two SMs, kCG = 2) per tile of 128 kCG rows x kBN
+// columns, persistent over the tiles:
+//   * warp 0 streams 64-deep pieces of A and B through a ring of stages by TMA
+//     (128-byte swizzle); a piece that passes the end of a matrix reads zeros;
+//   * warp 1 issues the products, K = 16 at a time, into one of two accumulators
+//     in tensor memory, so that
+//   * warps 2-5 read the other one (an output row per thread) and write the
+//     previous tile meanwhile.
+// A row tile starts at its group's first row and may reach into the next
+// group's rows: those outputs are not written.  Where the sum runs over the
+// rows (weight gradients) the last piece of a group is cleared behind the
+// group's last row in both operands (0 x inf would not be 0).
+//
+// A pair splits a tile by rows for A and the output and by columns for B, so each
+// SM loads half of B: 32 KB instead of 48 KB per 64-deep piece of 128 x 256
+// outputs per SM.
+//
+// Every wait on an mbarrier is bounded (wkv7_sync.cuh); a wait that runs out is
+// counted in camoe_wkv7_device_errors() and ends the roles' loops.
+#pragma once
+
+#include "wkv7_common.cuh"
+#include "wkv7_sync.cuh"
+#include "wkv7_tma.cuh"
+
+namespace camoe {
+namespace tc {
+
+constexpr int kBK = 64;           // depth of a stage: one 128-byte swizzled row of bf16
+constexpr int kThreads = 192;     // producer, product issue, four epilogue warps
+constexpr int kMaxGroups = 1025;  // 1024 and the rows of no group
+constexpr int kRingBytes = 192 * 1024;
+constexpr uint32_t kBox = 64 * 128;  // a box of 64 columns x 64 rows
+
+enum Epilogue : int {
+  kPlain = 0,   // out = acc
+  kRelu2 = 1,   // out = relu(acc)^2
+  kDRelu2 = 2,  // out = acc 2 sqrt(aux): the derivative of relu^2 from its value
+  kScale = 3,   // out = acc scale[group]
+};
+
+struct Args {
+  const int* offsets;    // [groups + 1]
+  int groups;
+  int64_t R;             // rows of A (the sorted arrays)
+  int M, N, K;           // M: weight gradients only
+  int K2, groups2;       // depth of the second pair, which groups below groups2 have
+  int b_shared;          // B is one matrix for all groups
+  int zero_tail;         // write zeros to the rows behind the last group
+  bf16* out;
+  const bf16* aux;       // [R, N] (kDRelu2)
+  const float* scale;    // [groups] or null (kScale)
+  const int* scatter;    // output row of row p, or null
+};
+
+template <int kCG, int kBN>
+struct Shape {
+  static constexpr int kBM = 128 * kCG;
+  static constexpr uint32_t kABytes = 128 * 128;          // per CTA and stage
+  static constexpr uint32_t kBBytes = kBN / kCG * 128;
+  static constexpr int kStages = kRingBytes / (kABytes + kBBytes) < 10 ? kRingBytes / (kABytes + kBBytes) : 10;
+  static constexpr uint32_t kCols = 2 * kBN;              // two accumulators
+};
+
+struct Control {
+  uint64_t full[10], empty[10], tail[10], acc_full[2], acc_empty[2], drained;
+  uint32_t tmem;
+  int tiles[kMaxGroups + 1];  // row tiles of the groups before each
+};
+
+template <int kCG, int kBN>
+__host__ __device__ constexpr int smem_bytes() {
+  return Shape<kCG, kBN>::kStages * static_cast<int>(Shape<kCG, kBN>::kABytes + Shape<kCG, kBN>::kBBytes) +
+         static_cast<int>(sizeof(Control)) + 1024;
+}
+
+// ---- PTX
+
+// mbarrier address in the CTA `rank` of the cluster (itself for a CTA alone)
+template <int kCG>
+__device__ __forceinline__ uint32_t bar_at(uint64_t* bar, uint32_t rank) {
+  uint32_t a = sm_addr(bar);
+  if (kCG > 1) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(rank));
+  return a;
+}
+template <int kCG>
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+  if (kCG > 1)
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+template <int kCG>
+__device__ __forceinline__ void expect_at(uint32_t bar, uint32_t bytes) {
+  if (kCG > 1)
+    asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar),
+                 "r"(bytes)
+                 : "memory");
+  else
+    asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+                 : "memory");
+}
+// bounded wait that also sees what the pair's other CTA wrote
+template <int kCG>
+__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity) {
+  if (kCG == 1) return mbar_wait(bar, parity);
+  long long t0 = 0, limit = 0;
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(sm_addr(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (limit == 0) {
+      t0 = clock64();
+      limit = *static_cast<volatile long long*>(&g_wkv7_wait_limit);
+    } else if (clock64() - t0 > limit) {
+      atomicAdd(&g_wkv7_timeouts, 1u);
+      return false;
+    }
+  }
+}
+// the whole warp waits, and leaves together when one of its lanes gave up
+template <int kCG>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, wait_on<kCG>(bar, parity));
+}
+// box at (x, y, z) into this CTA's shared memory, completing on the barrier at `bar`
+template <int kCG>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                         uint32_t bar) {
+  if (kCG > 1)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+template <int kCG>
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
+  if (kCG > 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm_addr(slot)),
+                 "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm_addr(slot)),
+                 "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+}
+template <int kCG>
+__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
+  if (kCG > 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+}
+template <int kCG>
+__device__ __forceinline__ void mma(uint32_t tmem, uint64_t da, uint64_t db, uint32_t idesc, bool add) {
+  if (kCG > 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem),
+        "l"(da), "l"(db), "r"(idesc), "r"(add ? 1u : 0u)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem),
+        "l"(da), "l"(db), "r"(idesc), "r"(add ? 1u : 0u)
+        : "memory");
+}
+// arrive on the barrier (in both CTAs of a pair) once the products issued so far are done
+template <int kCG>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if (kCG > 1)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            sm_addr(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sm_addr(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+template <int kCG>
+__device__ __forceinline__ void pair_sync() {
+  if (kCG > 1)
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  else
+    __syncthreads();
+}
+// 32 consecutive accumulator columns of this thread's TMEM lane
+__device__ __forceinline__ void ld32(uint32_t (&v)[32], uint32_t taddr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];\n"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
+        "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+        "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle (layout type 2), descriptor
+// version 1, 1024 bytes between groups of 8 rows.  K contiguous: the rows are M
+// (or N) and the leading offset is not used.  M (or N) contiguous: the rows are
+// K and the leading offset is the bytes between boxes of 64 columns.
+template <bool kMN>
+__device__ __forceinline__ uint64_t desc(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) |
+         (static_cast<uint64_t>(kMN ? (kBox >> 4) : 1u) << 16) | (static_cast<uint64_t>(1024u >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// bytes between K = 16 steps within a stage
+template <bool kMN>
+constexpr uint32_t kStep = kMN ? 16 * 128 : 32;
+
+// Instruction descriptor of kind::f16: fp32 accumulator, bf16 A and B, the
+// operands' majors (bits 15, 16: set for M or N contiguous), N / 8, M / 16.
+template <bool kAMN, bool kBMN>
+__host__ __device__ constexpr uint32_t instr(int M, int N) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (kAMN ? 1u << 15 : 0u) | (kBMN ? 1u << 16 : 0u) |
+         (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// ---- tiles
+
+struct Tile {
+  int group, n0;
+  int64_t row0, row1;  // the group's rows from the tile's first (weight gradients: all of the group's)
+  int m0;              // weight gradients: first output row
+  int nk1, nk;         // pieces of the first pair, of both
+};
+
+template <int kCG, int kBN, bool kWGrad>
+struct Tiles {
+  const Args& a;
+  const Control& c;
+  int nt, mt, total;
+  __device__ Tiles(const Args& args, const Control& ctl) : a(args), c(ctl) {
+    nt = (a.N + kBN - 1) / kBN;
+    mt = kWGrad ? (a.M + Shape<kCG, kBN>::kBM - 1) / Shape<kCG, kBN>::kBM : 0;
+    total = kWGrad ? a.groups * mt * nt : c.tiles[a.groups] * nt;
+  }
+  // rows are clamped to R: whatever the offsets hold, nothing outside the arrays is touched
+  __device__ int64_t first(int g) const {
+    const int64_t o = a.offsets[g];
+    return o < 0 ? 0 : (o < a.R ? o : a.R);
+  }
+  __device__ Tile get(int t) const {
+    Tile x;
+    const int rt = t / nt;
+    x.n0 = (t - rt * nt) * kBN;
+    if (kWGrad) {
+      x.group = rt / mt;
+      x.m0 = (rt - x.group * mt) * Shape<kCG, kBN>::kBM;
+      x.row0 = first(x.group);
+      x.row1 = first(x.group + 1);
+      x.nk1 = x.nk = x.row1 > x.row0 ? static_cast<int>((x.row1 - x.row0 + kBK - 1) / kBK) : 0;
+    } else {
+      int lo = 0, hi = a.groups;  // the last group whose first row tile is at most rt
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (c.tiles[mid] <= rt) lo = mid; else hi = mid;
+      }
+      x.group = lo;
+      x.m0 = 0;
+      x.row0 = first(lo) + static_cast<int64_t>(rt - c.tiles[lo]) * Shape<kCG, kBN>::kBM;
+      x.row1 = first(lo + 1);
+      x.nk1 = (a.K + kBK - 1) / kBK;
+      x.nk = x.nk1 + (lo < a.groups2 ? (a.K2 + kBK - 1) / kBK : 0);
+    }
+    return x;
+  }
+};
+
+template <int kEpi>
+__device__ __forceinline__ float finish(float x, float aux, float scale) {
+  if (kEpi == kRelu2) return x < 0.0f ? 0.0f : x * x;  // NaN stays NaN
+  if (kEpi == kDRelu2) return x * (2.0f * sqrtf(aux));
+  if (kEpi == kScale) return x * scale;
+  return x;
+}
+
+template <int kCG, int kBN, bool kAMN, bool kBMN, bool kWGrad, int kEpi>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
+                const __grid_constant__ CUtensorMap ma2, const __grid_constant__ CUtensorMap mb2,
+                const Args a) {
+  using Sh = Shape<kCG, kBN>;
+  constexpr int S = Sh::kStages, kBCols = kBN / kCG;
+  constexpr uint32_t kStage = Sh::kABytes + Sh::kBBytes;
+  extern __shared__ __align__(128) unsigned char raw[];
+  unsigned char* ring = raw + ((1024u - (sm_addr(raw) & 1023u)) & 1023u);
+  Control& c = *reinterpret_cast<Control*>(ring + S * kStage);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t rank = 0;
+  if (kCG > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int worker = blockIdx.x / kCG, workers = gridDim.x / kCG;
+
+  if (tid == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&c.full[s], kCG);
+      mbar_init(&c.empty[s], 1);
+      mbar_init(&c.tail[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&c.acc_full[b], 1);
+      mbar_init(&c.acc_empty[b], 4 * kCG);
+    }
+    mbar_init(&c.drained, 1);
+    mbar_fence_init();
+  }
+  if (warp == 1) tmem_alloc<kCG>(&c.tmem, Sh::kCols);
+  if (!kWGrad && warp == 2) {  // row tiles of each group
+    int carry = 0;
+    for (int g0 = 0; g0 < a.groups; g0 += 32) {
+      const int g = g0 + lane;
+      int n = 0;
+      if (g < a.groups) {
+        int64_t r0 = a.offsets[g], r1 = a.offsets[g + 1];
+        r0 = r0 < 0 ? 0 : (r0 < a.R ? r0 : a.R);
+        r1 = r1 < 0 ? 0 : (r1 < a.R ? r1 : a.R);
+        n = r1 > r0 ? static_cast<int>((r1 - r0 + Sh::kBM - 1) / Sh::kBM) : 0;
+      }
+      int x = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+      }
+      if (g < a.groups) c.tiles[g] = carry + x - n;
+      carry += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) c.tiles[a.groups] = carry;
+  }
+  fence_before();
+  __syncthreads();
+  if (kCG > 1) pair_sync<kCG>();
+  fence_after();
+  const uint32_t tmem = c.tmem, ring0 = sm_addr(ring);
+  const Tiles<kCG, kBN, kWGrad> tiles(a, c);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int i = 0;  // pieces loaded so far
+      bool ok = true;
+      for (int t = worker; ok && t < tiles.total; t += workers) {
+        const Tile x = tiles.get(t);
+        const int row = static_cast<int>(x.row0) + static_cast<int>(rank) * 128;
+        const int m = x.m0 + static_cast<int>(rank) * 128, n = x.n0 + static_cast<int>(rank) * kBCols;
+        const bool cut = kWGrad && ((x.row1 - x.row0) % kBK) != 0;
+        for (int j = 0; j < x.nk; ++j, ++i) {
+          const int s = i % S;
+          if (i >= S && !(ok = wait_on<kCG>(&c.empty[s], static_cast<uint32_t>((i / S - 1) & 1)))) break;
+          const bool last = cut && j == x.nk - 1;
+          // a piece to be cleared lands on this CTA's own barrier
+          const uint32_t bar = last ? sm_addr(&c.tail[s]) : bar_at<kCG>(&c.full[s], 0);
+          if (last)
+            mbar_arrive_expect_tx(&c.tail[s], kStage);
+          else
+            expect_at<kCG>(bar, kStage);
+          const uint32_t sa = ring0 + s * kStage, sb = sa + Sh::kABytes;
+          if (kWGrad) {
+            const int r = static_cast<int>(x.row0) + j * kBK;
+            load_box<kCG>(sa, &ma, m, r, 0, bar);
+            load_box<kCG>(sa + kBox, &ma, m + 64, r, 0, bar);
+#pragma unroll
+            for (int q = 0; q < kBCols / 64; ++q) load_box<kCG>(sb + q * kBox, &mb, n + 64 * q, r, 0, bar);
+          } else {
+            const bool one = j < x.nk1;
+            const int k = (one ? j : j - x.nk1) * kBK;
+            const CUtensorMap* pa = one ? &ma : &ma2;
+            const CUtensorMap* pb = one ? &mb : &mb2;
+            const int z = one && a.b_shared ? 0 : x.group;
+            load_box<kCG>(sa, pa, k, row, 0, bar);
+            if (kBMN) {
+#pragma unroll
+              for (int q = 0; q < kBCols / 64; ++q) load_box<kCG>(sb + q * kBox, pb, n + 64 * q, k, z, bar);
+            } else {
+              load_box<kCG>(sb, pb, k, n, z, bar);
+            }
+          }
+        }
+      }
+      // after a wait that ran out: this CTA's shared memory outlives the copies into it
+      if (!ok && rank == 0)
+        for (int q = i > S ? i - S : 0; q < i; ++q) wait_on<kCG>(&c.full[q % S], static_cast<uint32_t>((q / S) & 1));
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = instr<kAMN, kBMN>(Sh::kBM, kBN);
+    int i = 0, done = 0;
+    uint32_t tail_phase = 0;  // a bit per stage
+    bool ok = true;
+    for (int t = worker; ok && t < tiles.total; t += workers) {
+      const Tile x = tiles.get(t);
+      const int tail = kWGrad ? static_cast<int>((x.row1 - x.row0) % kBK) : 0;
+      if (x.nk == 0) continue;
+      const int b = done & 1;
+      if (rank == 0) {
+        if (done >= 2 && !(ok = warp_wait<kCG>(&c.acc_empty[b], static_cast<uint32_t>((done / 2 - 1) & 1)))) break;
+        fence_after();
+      }
+      for (int j = 0; j < x.nk; ++j, ++i) {
+        const int s = i % S;
+        const uint32_t sa = ring0 + s * kStage;
+        if (kWGrad && tail != 0 && j == x.nk - 1) {
+          if (!(ok = warp_wait<1>(&c.tail[s], (tail_phase >> s) & 1u))) break;
+          tail_phase ^= 1u << s;
+#pragma unroll 1
+          for (int q = 0; q < static_cast<int>(kStage / kBox); ++q)
+            for (uint32_t o = tail * 128 + lane * 16; o < kBox; o += 512)
+              *reinterpret_cast<uint4*>(ring + s * kStage + q * kBox + o) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) arrive_at<kCG>(bar_at<kCG>(&c.full[s], 0));
+        }
+        if (rank != 0) continue;
+        if (!(ok = warp_wait<kCG>(&c.full[s], static_cast<uint32_t>((i / S) & 1)))) break;
+        fence_after();
+        if (lane == 0) {
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k)
+            mma<kCG>(tmem + static_cast<uint32_t>(b * kBN), desc<kAMN>(sa + kStep<kAMN> * k),
+                     desc<kBMN>(sa + Sh::kABytes + kStep<kBMN> * k), idesc, j > 0 || k > 0);
+          commit<kCG>(&c.empty[s]);
+        }
+        __syncwarp();
+      }
+      if (rank == 0 && ok && lane == 0) commit<kCG>(&c.acc_full[b]);
+      __syncwarp();
+      ++done;
+    }
+    if (!ok && rank == 0 && lane == 0) {  // the products in flight end before tensor memory is freed
+      commit<kCG>(&c.drained);
+      wait_on<kCG>(&c.drained, 0);
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3;
+    int done = 0;
+    bool ok = true;
+    for (int t = worker; ok && t < tiles.total; t += workers) {
+      const Tile x = tiles.get(t);
+      const int b = done & 1;
+      const bool have = x.nk > 0;
+      if (have && !(ok = warp_wait<kCG>(&c.acc_full[b], static_cast<uint32_t>((done / 2) & 1)))) break;
+      fence_after();
+      const int in_tile = static_cast<int>(rank) * 128 + 32 * quarter + lane;
+      int64_t row;
+      bool mine;
+      if (kWGrad) {
+        row = static_cast<int64_t>(x.group) * a.M + x.m0 + in_tile;
+        mine = x.m0 + in_tile < a.M;
+      } else {
+        row = x.row0 + in_tile;
+        mine = row < x.row1;
+      }
+      const bf16* aux = kEpi == kDRelu2 ? a.aux + row * a.N : nullptr;
+      const float scale = kEpi == kScale && a.scale != nullptr ? a.scale[x.group] : 1.0f;
+      if (!kWGrad && a.scatter != nullptr && mine) row = a.scatter[row];
+      bf16* out = a.out + row * a.N;
+#pragma unroll 1
+      for (int c0 = 0; c0 < kBN; c0 += 32) {
+        if (x.n0 + c0 >= a.N) break;  // the same for the whole warp
+        uint32_t v[32];
+        __syncwarp();
+        if (have) {
+          ld32(v, tmem + (static_cast<uint32_t>(32 * quarter) << 16) + static_cast<uint32_t>(b * kBN + c0));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0u;
+        }
+        if (!mine) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = x.n0 + c0 + 8 * q;
+          if (n >= a.N) break;
+          uint4 av = make_uint4(0u, 0u, 0u, 0u);
+          if (kEpi == kDRelu2) av = *reinterpret_cast<const uint4*>(aux + n);
+          const __nv_bfloat162* ah = reinterpret_cast<const __nv_bfloat162*>(&av);
+          uint4 o;
+          __nv_bfloat162* oh = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 h = __bfloat1622float2(ah[e]);
+            oh[e] = __floats2bfloat162_rn(finish<kEpi>(__uint_as_float(v[8 * q + 2 * e]), h.x, scale),
+                                          finish<kEpi>(__uint_as_float(v[8 * q + 2 * e + 1]), h.y, scale));
+          }
+          *reinterpret_cast<uint4*>(out + n) = o;
+        }
+      }
+      if (have) {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_at<kCG>(bar_at<kCG>(&c.acc_empty[b], 0));
+        ++done;
+      }
+    }
+    if (!kWGrad && a.zero_tail) {
+      const int64_t pieces = a.N / 8;
+      const int64_t end = a.R * pieces;
+      uint4* out = reinterpret_cast<uint4*>(a.out);
+      const int64_t step = static_cast<int64_t>(gridDim.x) * 128;
+      for (int64_t i = tiles.first(a.groups) * pieces + static_cast<int64_t>(blockIdx.x) * 128 + (tid - 64); i < end;
+           i += step)
+        out[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (kCG > 1) pair_sync<kCG>();
+  if (warp == 1) tmem_free<kCG>(tmem, Sh::kCols);
+}
+
+}  // namespace tc
+}  // namespace camoe

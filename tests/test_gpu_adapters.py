@@ -1,0 +1,120 @@
+"""GPU numerics of the adapter projection (camoe_b200/adapters.py) against the
+formula in 64 bits.  A rounding to bf16 is at most 2^-8 of a value and below u =
+2^-9 in the root mean square; with few rows y is rounded once, with many the
+low-rank rows are rounded too: two roundings at most."""
+import pytest
+import torch
+
+from camoe_b200 import _lib, adapters
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+U = 2.0 ** -9
+
+
+@pytest.fixture(autouse=True)
+def _no_device_timeouts():
+    before = _lib.lib().camoe_wkv7_device_errors()
+    yield
+    assert _lib.lib().camoe_wkv7_device_errors() == before
+
+
+def rnd(*shape, seed, scale=1.0, dtype=BF):
+    return (scale * torch.randn(*shape, generator=torch.Generator().manual_seed(seed))).to(dtype).cuda()
+
+
+def inputs(N, C, M, D, L, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    adapter = torch.randint(-1, L, (N,), generator=g).to(torch.int32).cuda()
+    scale = (0.5 + torch.rand(L, generator=g)).cuda()
+    return (rnd(N, C, seed=seed + 1), rnd(M, C, seed=seed + 2, scale=C ** -0.5),
+            rnd(L, D, C, seed=seed + 3, scale=C ** -0.5), rnd(L, M, D, seed=seed + 4, scale=D ** -0.5), adapter, scale)
+
+
+def exact(x, weight, down, up, adapter, scale):
+    x = x.double()
+    y = x @ weight.double().t()
+    for a in range(down.shape[0]):
+        at = torch.nonzero(adapter == a)[:, 0]
+        s = 1.0 if scale is None else float(scale[a].double())
+        y[at] += s * ((x[at] @ down[a].double().t()) @ up[a].double().t())
+    return y
+
+
+def close(got, want, tol):
+    got = got.double()
+    assert torch.isfinite(got).all()
+    assert float((got - want).norm()) <= tol * float(want.norm())
+    typical = want.norm() / max(1, want.shape[0]) ** 0.5
+    assert float(((got - want).norm(dim=1) / torch.maximum(want.norm(dim=1), typical)).max()) <= 2 * tol
+
+
+CASES = [  # N, C, M, D, L
+    (1, 8, 8, 8, 1), (1, 1024, 1024, 16, 4), (7, 200, 72, 24, 3), (9, 64, 136, 40, 2), (33, 2048, 1000, 128, 64),
+    (256, 512, 512, 256, 5), (257, 64, 64, 8, 1), (300, 1000, 520, 16, 3), (400, 128, 256, 32, 64),
+    (1000, 264, 328, 96, 7), (2100, 512, 1032, 256, 2), (5000, 128, 128, 64, 40),
+]
+
+
+@pytest.mark.parametrize("N,C,M,D,L", CASES)
+def test_adapter_linear(N, C, M, D, L):
+    x, w, down, up, adapter, scale = inputs(N, C, M, D, L)
+    close(adapters.adapter_linear(x, w, down, up, adapter, scale), exact(x, w, down, up, adapter, scale), 2 * U)
+    close(adapters.adapter_linear(x, w, down, up, adapter), exact(x, w, down, up, adapter, None), 2 * U)
+
+
+@pytest.mark.parametrize("N", [20, 600])
+def test_rows_without_an_adapter_get_the_projection_alone(N):
+    x, w, down, up, adapter, scale = inputs(N, 128, 192, 16, 3, seed=10)
+    for none in (-1, 3, -2 ** 31, 2 ** 31 - 1):
+        adapter[:] = none
+        got = adapters.adapter_linear(x, w, down * float("nan"), up * float("nan"), adapter, scale)
+        close(got, x.double() @ w.double().t(), U * 1.01)
+    adapter[:] = 1  # one adapter for all, infinities in the others
+    down[0], up[2] = float("inf"), float("nan")
+    close(adapters.adapter_linear(x, w, down, up, adapter, scale),
+          exact(x, w, down[1:2], up[1:2], adapter - 1, scale[1:2]), 2 * U)
+
+
+@pytest.mark.parametrize("N", [50, 700])
+def test_a_row_of_infinities_stays_by_itself(N):
+    x, w, down, up, adapter, scale = inputs(N, 64, 128, 8, 4, seed=20)
+    clean = adapters.adapter_linear(x, w, down, up, adapter, scale)
+    bad = x.clone()
+    bad[5] = float("nan")
+    got = adapters.adapter_linear(bad, w, down, up, adapter, scale)
+    keep = torch.arange(N, device="cuda") != 5
+    assert torch.equal(got[keep], clean[keep]) and torch.isnan(got[5]).all()
+
+
+def test_empty_and_another_stream():
+    x, w, down, up, adapter, scale = inputs(500, 128, 256, 16, 5, seed=30)
+    first = adapters.adapter_linear(x, w, down, up, adapter, scale)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = adapters.adapter_linear(x, w, down, up, adapter, scale)
+    side.synchronize()
+    assert torch.equal(first, second)
+    assert adapters.adapter_linear(x[:0], w, down, up, adapter[:0], scale).shape == (0, 256)
+
+
+def test_refusals():
+    x, w, down, up, adapter, scale = inputs(4, 64, 32, 8, 2, seed=40)
+    call = adapters.adapter_linear
+    for kind, args in [
+        (TypeError, (x.float(), w, down, up, adapter, scale)),
+        (TypeError, (x, w, down, up, adapter.long(), scale)),
+        (TypeError, (x, w, down, up, adapter, scale.to(BF))),
+        (ValueError, (x, w, down, up[:1], adapter, scale)),
+        (ValueError, (x, w[:, :60].contiguous(), down, up, adapter, scale)),
+        (ValueError, (x, w, down[:, :4].contiguous(), up[:, :, :4].contiguous(), adapter, scale)),
+        (ValueError, (x, w, down, up, adapter[:3], scale)),
+        (ValueError, (x.cpu(), w, down, up, adapter, scale)),
+        (ValueError, (x.t().contiguous().t(), w, down, up, adapter, scale)),
+        (RuntimeError, (x, w.clone().requires_grad_(), down, up, adapter, scale)),
+    ]:
+        with pytest.raises(kind):
+            call(*args)
+    with torch.no_grad():
+        call(x, w.clone().requires_grad_(), down, up, adapter, scale)
