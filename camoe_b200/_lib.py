@@ -111,8 +111,8 @@ def lib() -> ctypes.CDLL:
     l.camoe_ex_dispatch.argtypes = [vp, ci, vp, ci] + [vp] * 5 + [sz] + [i64] * 4 + [vp]
     l.camoe_ex_combine.argtypes = [vp, ci] + [vp] * 3 + [i64] * 3 + [vp]
     l.camoe_ex_combine_bwd.argtypes = [vp, ci] + [vp] * 6 + [i64] * 4 + [vp]
-    l.camoe_ex_ffn_fwd.argtypes = [vp] * 6 + [i64] * 4 + [vp]
-    l.camoe_ex_ffn_bwd.argtypes = [vp] * 10 + [i64] * 4 + [vp]
+    l.camoe_ex_ffn_fwd.argtypes = [vp] * 7 + [i64] * 4 + [vp]
+    l.camoe_ex_ffn_bwd.argtypes = [vp] * 11 + [i64] * 4 + [vp]
     l.camoe_ad_work_bytes.restype = sz
     l.camoe_ad_work_bytes.argtypes = [i64] * 5
     l.camoe_ad_linear.argtypes = [vp] * 8 + [sz] + [i64] * 5 + [vp]

@@ -221,7 +221,7 @@ int camoe_ad_linear(const void* x, const void* weight, const void* down, const v
   a.out = static_cast<bf16*>(y);
   a.scale = nullptr;
   a.scatter = source;
-  return tc::launch<1, 256, false, false, false, tc::kPlain>({xs, C, N, 1}, {weight, C, M, 1}, {low, D, N, 1},
+  return tc::launch<2, 256, false, false, false, tc::kPlain>({xs, C, N, 1}, {weight, C, M, 1}, {low, D, N, 1},
                                                              {up, D, M, L}, a, s);
 }
 

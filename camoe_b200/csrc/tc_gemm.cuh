@@ -59,6 +59,7 @@ struct Args {
   int zero_tail;         // write zeros to the rows behind the last group
   bf16* out;
   const bf16* aux;       // [R, N] (kDRelu2)
+  int8_t* low;           // [R, N] (kRelu2, kDRelu2) or null: the 8 bits of the value below bf16's
   const float* scale;    // [groups] or null (kScale)
   const int* scatter;    // output row of row p, or null
 };
@@ -73,7 +74,7 @@ struct Shape {
 };
 
 struct Control {
-  uint64_t full[10], empty[10], tail[10], acc_full[2], acc_empty[2], drained;
+  uint64_t full[10], empty[10], tail[10], peer_tail[10], acc_full[2], acc_empty[2], drained;
   uint32_t tmem;
   int tiles[kMaxGroups + 1];  // row tiles of the groups before each
 };
@@ -93,27 +94,19 @@ __device__ __forceinline__ uint32_t bar_at(uint64_t* bar, uint32_t rank) {
   if (kCG > 1) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(rank));
   return a;
 }
-template <int kCG>
+// The scopes matter for speed: a release or an acquire at cluster scope waits
+// for the thread's memory traffic (0.8 us per stage of the ring when every
+// stage's barrier had them), and the ring needs none: TMA and the products order
+// themselves, and the epilogue's tcgen05 fences order tensor memory.  Only the
+// pieces that a CTA clears by ordinary stores are released to the pair's leader.
 __device__ __forceinline__ void arrive_at(uint32_t bar) {
-  if (kCG > 1)
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-  else
-    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-template <int kCG>
-__device__ __forceinline__ void expect_at(uint32_t bar, uint32_t bytes) {
-  if (kCG > 1)
-    asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar),
-                 "r"(bytes)
-                 : "memory");
-  else
-    asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-                 : "memory");
+__device__ __forceinline__ void arrive_release(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// bounded wait that also sees what the pair's other CTA wrote
-template <int kCG>
-__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity) {
-  if (kCG == 1) return mbar_wait(bar, parity);
+// bounded wait that sees what the pair's other CTA released
+__device__ __forceinline__ bool wait_acquire(uint64_t* bar, uint32_t parity) {
   long long t0 = 0, limit = 0;
   while (true) {
     uint32_t done;
@@ -134,9 +127,8 @@ __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity) {
   }
 }
 // the whole warp waits, and leaves together when one of its lanes gave up
-template <int kCG>
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, wait_on<kCG>(bar, parity));
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
 // box at (x, y, z) into this CTA's shared memory, completing on the barrier at `bar`
 template <int kCG>
@@ -301,13 +293,51 @@ struct Tiles {
   }
 };
 
+// A value as its bf16 rounding and 8 more bits: what an operand of the products
+// cannot hold but a derivative can use.
+__device__ __forceinline__ int low_bits(float v, bf16 hi) {
+  const int d = static_cast<int>(__float_as_uint(v) - (static_cast<uint32_t>(__bfloat16_as_ushort(hi)) << 16));
+  const int q = (d + 128) >> 8;
+  return q > 127 ? 127 : q;
+}
+__device__ __forceinline__ float with_low(float hi, int low) {
+  return __uint_as_float(__float_as_uint(hi) + (static_cast<uint32_t>(low) << 8));
+}
+// one instruction, 1 ulp: its result is multiplied and rounded to bf16
+__device__ __forceinline__ float fast_sqrt(float x) {
+  float y;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 template <int kEpi>
 __device__ __forceinline__ float finish(float x, float aux, float scale) {
   if (kEpi == kRelu2) return x < 0.0f ? 0.0f : x * x;  // NaN stays NaN
-  if (kEpi == kDRelu2) return x * (2.0f * sqrtf(aux));
+  if (kEpi == kDRelu2) return x * (2.0f * fast_sqrt(aux));
   if (kEpi == kScale) return x * scale;
   return x;
 }
+
+// What a thread reads of aux and low for 32 columns of its row
+struct Aux {
+  uint4 v[4], low[2];
+  template <int kEpi>
+  __device__ __forceinline__ void load(const Args& a, const bf16* aux, const int8_t* low_row, int n, bool mine) {
+    if (kEpi != kDRelu2) return;
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      v[q] = mine && n + 8 * q < a.N ? *reinterpret_cast<const uint4*>(aux + n + 8 * q) : zero;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {  // N is a multiple of 8: 16 bytes, or the last 8
+      low[q] = zero;
+      const int m = n + 16 * q;
+      if (a.low == nullptr || !mine || m >= a.N) continue;
+      const uint2 x = *reinterpret_cast<const uint2*>(low_row + m);
+      const uint2 y = m + 8 < a.N ? *reinterpret_cast<const uint2*>(low_row + m + 8) : make_uint2(0u, 0u);
+      low[q] = make_uint4(x.x, x.y, y.x, y.y);
+    }
+  }
+};
 
 template <int kCG, int kBN, bool kAMN, bool kBMN, bool kWGrad, int kEpi>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -327,9 +357,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&c.full[s], kCG);
+      mbar_init(&c.full[s], 1);
       mbar_init(&c.empty[s], 1);
       mbar_init(&c.tail[s], 1);
+      mbar_init(&c.peer_tail[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&c.acc_full[b], 1);
@@ -379,14 +410,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool cut = kWGrad && ((x.row1 - x.row0) % kBK) != 0;
         for (int j = 0; j < x.nk; ++j, ++i) {
           const int s = i % S;
-          if (i >= S && !(ok = wait_on<kCG>(&c.empty[s], static_cast<uint32_t>((i / S - 1) & 1)))) break;
+          if (i >= S && !(ok = mbar_wait(&c.empty[s], static_cast<uint32_t>((i / S - 1) & 1)))) break;
           const bool last = cut && j == x.nk - 1;
           // a piece to be cleared lands on this CTA's own barrier
           const uint32_t bar = last ? sm_addr(&c.tail[s]) : bar_at<kCG>(&c.full[s], 0);
           if (last)
             mbar_arrive_expect_tx(&c.tail[s], kStage);
-          else
-            expect_at<kCG>(bar, kStage);
+          else if (rank == 0)  // for both CTAs: the pair's loads complete on the leader's barrier
+            mbar_arrive_expect_tx(&c.full[s], kCG * kStage);
           const uint32_t sa = ring0 + s * kStage, sb = sa + Sh::kABytes;
           if (kWGrad) {
             const int r = static_cast<int>(x.row0) + j * kBK;
@@ -412,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // after a wait that ran out: this CTA's shared memory outlives the copies into it
       if (!ok && rank == 0)
-        for (int q = i > S ? i - S : 0; q < i; ++q) wait_on<kCG>(&c.full[q % S], static_cast<uint32_t>((q / S) & 1));
+        for (int q = i > S ? i - S : 0; q < i; ++q) mbar_wait(&c.full[q % S], static_cast<uint32_t>((q / S) & 1));
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc = instr<kAMN, kBMN>(Sh::kBM, kBN);
@@ -425,14 +456,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (x.nk == 0) continue;
       const int b = done & 1;
       if (rank == 0) {
-        if (done >= 2 && !(ok = warp_wait<kCG>(&c.acc_empty[b], static_cast<uint32_t>((done / 2 - 1) & 1)))) break;
+        if (done >= 2 && !(ok = warp_wait(&c.acc_empty[b], static_cast<uint32_t>((done / 2 - 1) & 1)))) break;
         fence_after();
       }
       for (int j = 0; j < x.nk; ++j, ++i) {
         const int s = i % S;
         const uint32_t sa = ring0 + s * kStage;
         if (kWGrad && tail != 0 && j == x.nk - 1) {
-          if (!(ok = warp_wait<1>(&c.tail[s], (tail_phase >> s) & 1u))) break;
+          if (!(ok = warp_wait(&c.tail[s], (tail_phase >> s) & 1u))) break;
           tail_phase ^= 1u << s;
 #pragma unroll 1
           for (int q = 0; q < static_cast<int>(kStage / kBox); ++q)
@@ -440,10 +471,18 @@ __global__ void __launch_bounds__(kThreads, 1)
               *reinterpret_cast<uint4*>(ring + s * kStage + q * kBox + o) = make_uint4(0u, 0u, 0u, 0u);
           fence_proxy_async();
           __syncwarp();
-          if (lane == 0) arrive_at<kCG>(bar_at<kCG>(&c.full[s], 0));
+          if (kCG > 1 && rank != 0) {
+            if (lane == 0) arrive_release(bar_at<kCG>(&c.peer_tail[s], 0));
+          } else {
+            if (kCG > 1 &&
+                !(ok = __all_sync(0xffffffffu, wait_acquire(&c.peer_tail[s], ((tail_phase >> s) & 1u) ^ 1u))))
+              break;
+            if (lane == 0) mbar_arrive(&c.full[s]);  // the stage's phase, which no load completes
+            __syncwarp();
+          }
         }
         if (rank != 0) continue;
-        if (!(ok = warp_wait<kCG>(&c.full[s], static_cast<uint32_t>((i / S) & 1)))) break;
+        if (!(ok = warp_wait(&c.full[s], static_cast<uint32_t>((i / S) & 1)))) break;
         fence_after();
         if (lane == 0) {
 #pragma unroll
@@ -460,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!ok && rank == 0 && lane == 0) {  // the products in flight end before tensor memory is freed
       commit<kCG>(&c.drained);
-      wait_on<kCG>(&c.drained, 0);
+      mbar_wait(&c.drained, 0);
     }
     __syncwarp();
   } else {
@@ -471,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Tile x = tiles.get(t);
       const int b = done & 1;
       const bool have = x.nk > 0;
-      if (have && !(ok = warp_wait<kCG>(&c.acc_full[b], static_cast<uint32_t>((done / 2) & 1)))) break;
+      if (have && !(ok = warp_wait(&c.acc_full[b], static_cast<uint32_t>((done / 2) & 1)))) break;
       fence_after();
       const int in_tile = static_cast<int>(rank) * 128 + 32 * quarter + lane;
       int64_t row;
@@ -484,12 +523,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         mine = row < x.row1;
       }
       const bf16* aux = kEpi == kDRelu2 ? a.aux + row * a.N : nullptr;
+      int8_t* low_row = kEpi == kRelu2 || kEpi == kDRelu2 ? a.low + (a.low != nullptr ? row * a.N : 0) : nullptr;
       const float scale = kEpi == kScale && a.scale != nullptr ? a.scale[x.group] : 1.0f;
       if (!kWGrad && a.scatter != nullptr && mine) row = a.scatter[row];
       bf16* out = a.out + row * a.N;
+      Aux next;  // loaded a step ahead: a step is shorter than a load takes
+      next.load<kEpi>(a, aux, low_row, x.n0, mine);
 #pragma unroll 1
       for (int c0 = 0; c0 < kBN; c0 += 32) {
         if (x.n0 + c0 >= a.N) break;  // the same for the whole warp
+        const Aux now = next;
+        if (c0 + 32 < kBN) next.load<kEpi>(a, aux, low_row, x.n0 + c0 + 32, mine);
         uint32_t v[32];
         __syncwarp();
         if (have) {
@@ -503,24 +547,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int q = 0; q < 4; ++q) {
           const int n = x.n0 + c0 + 8 * q;
           if (n >= a.N) break;
-          uint4 av = make_uint4(0u, 0u, 0u, 0u);
-          if (kEpi == kDRelu2) av = *reinterpret_cast<const uint4*>(aux + n);
-          const __nv_bfloat162* ah = reinterpret_cast<const __nv_bfloat162*>(&av);
+          const bf16* ah = reinterpret_cast<const bf16*>(&now.v[q]);
+          const int8_t* al = reinterpret_cast<const int8_t*>(&now.low[q / 2]) + 8 * (q % 2);
           uint4 o;
+          uint2 l;
           __nv_bfloat162* oh = reinterpret_cast<__nv_bfloat162*>(&o);
+          int8_t* ol = reinterpret_cast<int8_t*>(&l);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 h = __bfloat1622float2(ah[e]);
-            oh[e] = __floats2bfloat162_rn(finish<kEpi>(__uint_as_float(v[8 * q + 2 * e]), h.x, scale),
-                                          finish<kEpi>(__uint_as_float(v[8 * q + 2 * e + 1]), h.y, scale));
+            float h0 = 0.0f, h1 = 0.0f;
+            if (kEpi == kDRelu2) {
+              h0 = with_low(__bfloat162float(ah[2 * e]), al[2 * e]);
+              h1 = with_low(__bfloat162float(ah[2 * e + 1]), al[2 * e + 1]);
+            }
+            const float y0 = finish<kEpi>(__uint_as_float(v[8 * q + 2 * e]), h0, scale);
+            const float y1 = finish<kEpi>(__uint_as_float(v[8 * q + 2 * e + 1]), h1, scale);
+            oh[e] = __floats2bfloat162_rn(y0, y1);
+            if (kEpi == kRelu2) {
+              ol[2 * e] = static_cast<int8_t>(low_bits(y0, oh[e].x));
+              ol[2 * e + 1] = static_cast<int8_t>(low_bits(y1, oh[e].y));
+            }
           }
           *reinterpret_cast<uint4*>(out + n) = o;
+          if (kEpi == kRelu2 && a.low != nullptr) *reinterpret_cast<uint2*>(low_row + n) = l;
         }
       }
       if (have) {
         fence_before();
         __syncwarp();
-        if (lane == 0) arrive_at<kCG>(bar_at<kCG>(&c.acc_empty[b], 0));
+        if (lane == 0) arrive_at(bar_at<kCG>(&c.acc_empty[b], 0));
         ++done;
       }
     }

@@ -169,26 +169,29 @@ def expert_combine(ys: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan) -> 
     return _combine(ys, weight, plan.position, ys.shape[1])
 
 
-def _ffn(xs, w_up, w_down, offsets):
+def _ffn(xs, w_up, w_down, offsets, low: bool):
     R, C = xs.shape
     E, F, _ = w_up.shape
     h = torch.empty(R, F, dtype=xs.dtype, device=xs.device)
+    h_low = torch.empty(R, F, dtype=torch.int8, device=xs.device) if low else None
     ys = torch.empty(R, C, dtype=xs.dtype, device=xs.device)
     check(_lib.lib().camoe_ex_ffn_fwd(xs.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), offsets.data_ptr(),
-                                      h.data_ptr(), ys.data_ptr(), R, E, C, F, _stream(xs)))
-    return ys, h
+                                      h.data_ptr(), None if h_low is None else h_low.data_ptr(), ys.data_ptr(), R, E, C, F,
+                                      _stream(xs)))
+    return ys, h, h_low
 
 
 class _FfnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, xs, w_up, w_down, offsets):
-        ys, h = _ffn(xs, w_up, w_down, offsets)
-        ctx.save_for_backward(xs, w_up, w_down, offsets, h)
+        # h to 8 bits below bf16 where the backward takes its root
+        ys, h, h_low = _ffn(xs, w_up, w_down, offsets, ctx.needs_input_grad[0] or ctx.needs_input_grad[1])
+        ctx.save_for_backward(xs, w_up, w_down, offsets, h, h_low)
         return ys
 
     @staticmethod
     def backward(ctx, dys):
-        xs, w_up, w_down, offsets, h = ctx.saved_tensors
+        xs, w_up, w_down, offsets, h, h_low = ctx.saved_tensors
         dys = dys.contiguous()
         R, C = xs.shape
         E, F, _ = w_up.shape
@@ -198,7 +201,7 @@ class _FfnFn(torch.autograd.Function):
         ptr = (lambda t: None if t is None else t.data_ptr())
         check(_lib.lib().camoe_ex_ffn_bwd(
             dys.data_ptr(), xs.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), offsets.data_ptr(), h.data_ptr(),
-            ptr(dpre), ptr(dxs), ptr(dw_up), ptr(dw_down), R, E, C, F, _stream(xs)))
+            ptr(h_low), ptr(dpre), ptr(dxs), ptr(dw_up), ptr(dw_down), R, E, C, F, _stream(xs)))
         return dxs, dw_up, dw_down, None
 
 
@@ -225,4 +228,4 @@ def expert_ffn(xs: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, offse
         raise ValueError(f"the widths must be positive multiples of 8, got C = {C} and F = {F}")
     if torch.is_grad_enabled() and (xs.requires_grad or w_up.requires_grad or w_down.requires_grad):
         return _FfnFn.apply(xs, w_up, w_down, offsets)
-    return _ffn(xs, w_up, w_down, offsets)[0]
+    return _ffn(xs, w_up, w_down, offsets, False)[0]

@@ -56,17 +56,19 @@ int camoe_ex_combine_bwd(const void* dout, int dtype, const void* ys, const floa
 /* The experts' products over sorted rows, bf16: for the rows p of expert e
  *   h[p]  = relu(w_up[e] xs[p])^2      w_up   [E, F, C]
  *   ys[p] = w_down[e] h[p]             w_down [E, C, F]
- * h [R, F] is written too (the backward's input); the rows behind offsets[E]
- * of ys are zeros.  C and F are multiples of 8. */
+ * h [R, F] is written too, and h_low [R, F] (bytes, may be NULL): the 8 bits of
+ * h below bf16's, for the backward.  The rows behind offsets[E] of ys are zeros.
+ * C and F are multiples of 8. */
 int camoe_ex_ffn_fwd(const void* xs, const void* w_up, const void* w_down, const int32_t* offsets,
-                     void* h, void* ys, int64_t R, int64_t E, int64_t C, int64_t F, void* stream);
+                     void* h, void* h_low, void* ys, int64_t R, int64_t E, int64_t C, int64_t F, void* stream);
 
 /* Backward of camoe_ex_ffn_fwd: dpre [R, F] is scratch; dxs [R, C], dw_up
- * [E, F, C] and dw_down [E, C, F] are bf16 and each may be NULL.  An expert
- * without rows gets zero weight gradients. */
+ * [E, F, C] and dw_down [E, C, F] are bf16 and each may be NULL.  h and h_low
+ * are the forward's (h_low may be NULL: h as rounded to bf16 is used alone).  An
+ * expert without rows gets zero weight gradients. */
 int camoe_ex_ffn_bwd(const void* dys, const void* xs, const void* w_up, const void* w_down,
-                     const int32_t* offsets, const void* h, void* dpre, void* dxs, void* dw_up,
-                     void* dw_down, int64_t R, int64_t E, int64_t C, int64_t F, void* stream);
+                     const int32_t* offsets, const void* h, const void* h_low, void* dpre, void* dxs,
+                     void* dw_up, void* dw_down, int64_t R, int64_t E, int64_t C, int64_t F, void* stream);
 
 /* Bytes of workspace of camoe_ad_linear. */
 size_t camoe_ad_work_bytes(int64_t N, int64_t C, int64_t M, int64_t D, int64_t L);

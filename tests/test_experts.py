@@ -55,7 +55,7 @@ def test_combine_statuses():
 
 
 def ffn(R=4, E=2, C=16, F=32, offsets=P, xs=P):
-    return _lib.lib().camoe_ex_ffn_fwd(xs, P, P, offsets, P, P, R, E, C, F, None)
+    return _lib.lib().camoe_ex_ffn_fwd(xs, P, P, offsets, P, P, P, R, E, C, F, None)
 
 
 def test_ffn_statuses():
@@ -67,8 +67,8 @@ def test_ffn_statuses():
     assert ffn(xs=P + 2) == _lib.ERR_ALIGNMENT
     assert ffn(R=0) == _lib.OK
     b = _lib.lib().camoe_ex_ffn_bwd
-    assert b(P + 4, *[P] * 9, 4, 2, 16, 32, None) == _lib.ERR_ALIGNMENT
-    assert b(None, *[P] * 9, 4, 2, 16, 32, None) == _lib.ERR_INVALID_ARG
+    assert b(P + 4, *[P] * 10, 4, 2, 16, 32, None) == _lib.ERR_ALIGNMENT
+    assert b(None, *[P] * 10, 4, 2, 16, 32, None) == _lib.ERR_INVALID_ARG
 
 
 def test_adapter_statuses():
