@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(thin::kThreads) thin_kernel(const bf16* __rest
         if (kRelu2) v = v < 0.0f ? 0.0f : v * v;
         const bf16 hi = __float2bfloat16_rn(v);
         out[(p + r) * O + o0 + o] = hi;
-        if (kRelu2 && low != nullptr) low[(p + r) * O + o0 + o] = static_cast<int8_t>(tc::low_bits(v, hi));
+        if (kRelu2 && low != nullptr) low[(p + r) * tc::low_stride(O) + o0 + o] = static_cast<int8_t>(tc::low_bits(v, hi));
       }
     }
     __syncthreads();  // red is written again
@@ -124,11 +124,13 @@ tc::Args args(const int* offsets, int64_t E, int64_t R, int64_t N, int64_t K, vo
   return a;
 }
 
-// rows x grouped weights; w is [E][N][K], or [E][K][N] where kBMN
+// rows x grouped weights; w is [E][N][K], or [E][K][N] where kBMN; h for kDRelu2
 template <bool kBMN, int kEpi>
-int rows_product(const void* x, const void* w, const tc::Args& a, int64_t E, cudaStream_t st) {
+int rows_product(const void* x, const void* w, const tc::Args& a, int64_t E, cudaStream_t st,
+                 const void* h = nullptr) {
   return tc::launch<2, 256, false, kBMN, false, kEpi>(
-      {x, a.K, a.R, 1}, kBMN ? tc::Matrix{w, a.N, a.K, E} : tc::Matrix{w, a.K, a.N, E}, {}, {}, a, st);
+      {x, a.K, a.R, 1}, kBMN ? tc::Matrix{w, a.N, a.K, E} : tc::Matrix{w, a.K, a.N, E}, {h, a.N, a.R, 1},
+      {}, a, st);
 }
 
 int check(const int* offsets, int64_t R, int64_t E, int64_t C, int64_t F) {
@@ -193,9 +195,8 @@ int camoe_ex_ffn_bwd(const void* dys, const void* xs, const void* w_up, const vo
   if (dxs != nullptr || dw_up != nullptr) {
     if (w_down == nullptr || dpre == nullptr) return 1;
     tc::Args a = args(offsets, E, R, F, C, dpre);
-    a.aux = static_cast<const bf16*>(h);
     a.low = static_cast<int8_t*>(const_cast<void*>(h_low));  // read only
-    if (const int st = rows_product<true, tc::kDRelu2>(dys, w_down, a, E, s)) return st;
+    if (const int st = rows_product<true, tc::kDRelu2>(dys, w_down, a, E, s, h)) return st;
   }
   if (dxs != nullptr) {
     if (w_up == nullptr) return 1;

@@ -15,7 +15,8 @@
 //   * warp 1 issues the products, K = 16 at a time, into one of two accumulators
 //     in tensor memory, so that
 //   * warps 2-5 read the other one (an output row per thread) and write the
-//     previous tile meanwhile.
+//     previous tile meanwhile, turned through shared memory so that a warp's
+//     stores (and its loads of h) are whole 128-byte row segments.
 // A row tile starts at its group's first row and may reach into the next
 // group's rows: those outputs are not written.  Where the sum runs over the
 // rows (weight gradients) the last piece of a group is cleared behind the
@@ -45,9 +46,12 @@ constexpr uint32_t kBox = 64 * 128;  // a box of 64 columns x 64 rows
 enum Epilogue : int {
   kPlain = 0,   // out = acc
   kRelu2 = 1,   // out = relu(acc)^2
-  kDRelu2 = 2,  // out = acc 2 sqrt(aux): the derivative of relu^2 from its value
+  kDRelu2 = 2,  // out = acc 2 sqrt(h): the derivative of relu^2 from its value (maps ma2: h, mb2: low)
   kScale = 3,   // out = acc scale[group]
 };
+
+// rows of low start at multiples of 16 bytes
+__host__ __device__ constexpr int64_t low_stride(int64_t n) { return (n + 15) / 16 * 16; }
 
 struct Args {
   const int* offsets;    // [groups + 1]
@@ -58,30 +62,37 @@ struct Args {
   int b_shared;          // B is one matrix for all groups
   int zero_tail;         // write zeros to the rows behind the last group
   bf16* out;
-  const bf16* aux;       // [R, N] (kDRelu2)
-  int8_t* low;           // [R, N] (kRelu2, kDRelu2) or null: the 8 bits of the value below bf16's
+  int8_t* low;           // [R, low_stride(N)] (kRelu2, kDRelu2) or null: the 8 bits of the value below bf16's
   const float* scale;    // [groups] or null (kScale)
   const int* scatter;    // output row of row p, or null
 };
 
-template <int kCG, int kBN>
+// Per epilogue warp: 32 rows x 64 columns of bf16, and of bytes
+constexpr uint32_t kOutBytes = 32 * 128, kLowBytes = 32 * 64;
+
+template <int kCG, int kBN, int kEpi>
 struct Shape {
   static constexpr int kBM = 128 * kCG;
   static constexpr uint32_t kABytes = 128 * 128;          // per CTA and stage
   static constexpr uint32_t kBBytes = kBN / kCG * 128;
-  static constexpr int kStages = kRingBytes / (kABytes + kBBytes) < 10 ? kRingBytes / (kABytes + kBBytes) : 10;
+  // kDRelu2 reads h a step ahead: two staging buffers per warp, in place of a stage
+  static constexpr int kBufs = kEpi == kDRelu2 ? 2 : 1;
+  static constexpr int kFit = (kRingBytes - (kBufs - 1) * 32 * 1024) / (kABytes + kBBytes);
+  static constexpr int kStages = kFit < 10 ? kFit : 10;
+  static constexpr uint32_t kStaging = 4 * kBufs * (kOutBytes + kLowBytes);
   static constexpr uint32_t kCols = 2 * kBN;              // two accumulators
 };
 
 struct Control {
-  uint64_t full[10], empty[10], tail[10], peer_tail[10], acc_full[2], acc_empty[2], drained;
+  uint64_t full[10], empty[10], tail[10], peer_tail[10], acc_full[2], acc_empty[2], drained, aux[4][2];
   uint32_t tmem;
   int tiles[kMaxGroups + 1];  // row tiles of the groups before each
 };
 
-template <int kCG, int kBN>
+template <int kCG, int kBN, int kEpi>
 __host__ __device__ constexpr int smem_bytes() {
-  return Shape<kCG, kBN>::kStages * static_cast<int>(Shape<kCG, kBN>::kABytes + Shape<kCG, kBN>::kBBytes) +
+  using Sh = Shape<kCG, kBN, kEpi>;
+  return Sh::kStages * static_cast<int>(Sh::kABytes + Sh::kBBytes) + static_cast<int>(Sh::kStaging) +
          static_cast<int>(sizeof(Control)) + 1024;
 }
 
@@ -205,19 +216,25 @@ __device__ __forceinline__ void pair_sync() {
   else
     __syncthreads();
 }
-// 32 consecutive accumulator columns of this thread's TMEM lane
-__device__ __forceinline__ void ld32(uint32_t (&v)[32], uint32_t taddr) {
+// 64 consecutive accumulator columns of this thread's TMEM lane (the wait is in the
+// same statement, so that no use of v can be moved before it)
+__device__ __forceinline__ void ld64(uint32_t (&v)[64], uint32_t taddr) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-      "%30, %31}, [%32];\n"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
-        "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
-        "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]),
+        "=r"(v[32]), "=r"(v[33]), "=r"(v[34]), "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]),
+        "=r"(v[40]), "=r"(v[41]), "=r"(v[42]), "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]),
+        "=r"(v[48]), "=r"(v[49]), "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]),
+        "=r"(v[56]), "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63])
+      : "r"(taddr)
+      : "memory");
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle (layout type 2), descriptor
@@ -258,7 +275,7 @@ struct Tiles {
   int nt, mt, total;
   __device__ Tiles(const Args& args, const Control& ctl) : a(args), c(ctl) {
     nt = (a.N + kBN - 1) / kBN;
-    mt = kWGrad ? (a.M + Shape<kCG, kBN>::kBM - 1) / Shape<kCG, kBN>::kBM : 0;
+    mt = kWGrad ? (a.M + (128 * kCG) - 1) / (128 * kCG) : 0;
     total = kWGrad ? a.groups * mt * nt : c.tiles[a.groups] * nt;
   }
   // rows are clamped to R: whatever the offsets hold, nothing outside the arrays is touched
@@ -272,7 +289,7 @@ struct Tiles {
     x.n0 = (t - rt * nt) * kBN;
     if (kWGrad) {
       x.group = rt / mt;
-      x.m0 = (rt - x.group * mt) * Shape<kCG, kBN>::kBM;
+      x.m0 = (rt - x.group * mt) * (128 * kCG);
       x.row0 = first(x.group);
       x.row1 = first(x.group + 1);
       x.nk1 = x.nk = x.row1 > x.row0 ? static_cast<int>((x.row1 - x.row0 + kBK - 1) / kBK) : 0;
@@ -284,7 +301,7 @@ struct Tiles {
       }
       x.group = lo;
       x.m0 = 0;
-      x.row0 = first(lo) + static_cast<int64_t>(rt - c.tiles[lo]) * Shape<kCG, kBN>::kBM;
+      x.row0 = first(lo) + static_cast<int64_t>(rt - c.tiles[lo]) * (128 * kCG);
       x.row1 = first(lo + 1);
       x.nk1 = (a.K + kBK - 1) / kBK;
       x.nk = x.nk1 + (lo < a.groups2 ? (a.K2 + kBK - 1) / kBK : 0);
@@ -317,39 +334,23 @@ __device__ __forceinline__ float finish(float x, float aux, float scale) {
   return x;
 }
 
-// What a thread reads of aux and low for 32 columns of its row
-struct Aux {
-  uint4 v[4], low[2];
-  template <int kEpi>
-  __device__ __forceinline__ void load(const Args& a, const bf16* aux, const int8_t* low_row, int n, bool mine) {
-    if (kEpi != kDRelu2) return;
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      v[q] = mine && n + 8 * q < a.N ? *reinterpret_cast<const uint4*>(aux + n + 8 * q) : zero;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {  // N is a multiple of 8: 16 bytes, or the last 8
-      low[q] = zero;
-      const int m = n + 16 * q;
-      if (a.low == nullptr || !mine || m >= a.N) continue;
-      const uint2 x = *reinterpret_cast<const uint2*>(low_row + m);
-      const uint2 y = m + 8 < a.N ? *reinterpret_cast<const uint2*>(low_row + m + 8) : make_uint2(0u, 0u);
-      low[q] = make_uint4(x.x, x.y, y.x, y.y);
-    }
-  }
-};
+// 16-byte piece q of row r in a warp's staging buffers: swizzled, so that both a
+// thread per row and eight (four) threads per row touch all banks
+__device__ __forceinline__ uint32_t out_at(int r, int q) { return r * 128 + ((q ^ (r & 7)) << 4); }
+__device__ __forceinline__ uint32_t low_at(int r, int q) { return r * 64 + ((q ^ ((r >> 1) & 3)) << 4); }
 
 template <int kCG, int kBN, bool kAMN, bool kBMN, bool kWGrad, int kEpi>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
                 const __grid_constant__ CUtensorMap ma2, const __grid_constant__ CUtensorMap mb2,
                 const Args a) {
-  using Sh = Shape<kCG, kBN>;
+  using Sh = Shape<kCG, kBN, kEpi>;
   constexpr int S = Sh::kStages, kBCols = kBN / kCG;
   constexpr uint32_t kStage = Sh::kABytes + Sh::kBBytes;
   extern __shared__ __align__(128) unsigned char raw[];
   unsigned char* ring = raw + ((1024u - (sm_addr(raw) & 1023u)) & 1023u);
-  Control& c = *reinterpret_cast<Control*>(ring + S * kStage);
+  unsigned char* staging = ring + S * kStage;
+  Control& c = *reinterpret_cast<Control*>(staging + Sh::kStaging);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint32_t rank = 0;
   if (kCG > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -367,6 +368,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&c.acc_empty[b], 4 * kCG);
     }
     mbar_init(&c.drained, 1);
+    for (int w = 0; w < 4; ++w)
+      for (int b = 0; b < Sh::kBufs; ++b) mbar_init(&c.aux[w][b], 1);
     mbar_fence_init();
   }
   if (warp == 1) tmem_alloc<kCG>(&c.tmem, Sh::kCols);
@@ -504,55 +507,73 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else {
     const int quarter = warp & 3;
+    unsigned char* outs = staging + quarter * (Sh::kBufs * kOutBytes);
+    unsigned char* all_lows = staging + 4 * Sh::kBufs * kOutBytes + quarter * (Sh::kBufs * kLowBytes);
+    int steps = 0, asked = 0;  // kDRelu2: boxes of h this warp has read, and asked for
+    const auto fetch = [&](int step, int n, int64_t row) {  // 64 columns of h and low
+      asked = step + 1;
+      if (lane != 0) return;
+      uint64_t* bar = &c.aux[quarter][step & 1];
+      mbar_arrive_expect_tx(bar, kOutBytes + (a.low != nullptr ? kLowBytes : 0));
+      load_box<1>(sm_addr(outs + (step & 1) * kOutBytes), &ma2, n, static_cast<int>(row), 0, sm_addr(bar));
+      if (a.low != nullptr)
+        load_box<1>(sm_addr(all_lows + (step & 1) * kLowBytes), &mb2, n, static_cast<int>(row), 0, sm_addr(bar));
+    };
     int done = 0;
     bool ok = true;
     for (int t = worker; ok && t < tiles.total; t += workers) {
       const Tile x = tiles.get(t);
       const int b = done & 1;
       const bool have = x.nk > 0;
+      // the warp's 32 rows: the first, and how many of them exist
+      const int in_tile = static_cast<int>(rank) * 128 + 32 * quarter;
+      const int64_t row0 = (kWGrad ? static_cast<int64_t>(x.group) * a.M + x.m0 : x.row0) + in_tile;
+      const int64_t left = (kWGrad ? a.M - x.m0 : x.row1 - x.row0) - in_tile;
+      const int rows = left < 32 ? (left > 0 ? static_cast<int>(left) : 0) : 32;
+      const float scale = kEpi == kScale && a.scale != nullptr ? a.scale[x.group] : 1.0f;
+      int to = 0;  // where this lane's row goes
+      if (!kWGrad && a.scatter != nullptr && lane < rows) to = a.scatter[row0 + lane];
+      if (kEpi == kDRelu2 && rows > 0) fetch(steps, x.n0, row0);
       if (have && !(ok = warp_wait(&c.acc_full[b], static_cast<uint32_t>((done / 2) & 1)))) break;
       fence_after();
-      const int in_tile = static_cast<int>(rank) * 128 + 32 * quarter + lane;
-      int64_t row;
-      bool mine;
-      if (kWGrad) {
-        row = static_cast<int64_t>(x.group) * a.M + x.m0 + in_tile;
-        mine = x.m0 + in_tile < a.M;
-      } else {
-        row = x.row0 + in_tile;
-        mine = row < x.row1;
-      }
-      const bf16* aux = kEpi == kDRelu2 ? a.aux + row * a.N : nullptr;
-      int8_t* low_row = kEpi == kRelu2 || kEpi == kDRelu2 ? a.low + (a.low != nullptr ? row * a.N : 0) : nullptr;
-      const float scale = kEpi == kScale && a.scale != nullptr ? a.scale[x.group] : 1.0f;
-      if (!kWGrad && a.scatter != nullptr && mine) row = a.scatter[row];
-      bf16* out = a.out + row * a.N;
-      Aux next;  // loaded a step ahead: a step is shorter than a load takes
-      next.load<kEpi>(a, aux, low_row, x.n0, mine);
+      const int cols = a.N - x.n0 < kBN ? a.N - x.n0 : kBN;
 #pragma unroll 1
-      for (int c0 = 0; c0 < kBN; c0 += 32) {
-        if (x.n0 + c0 >= a.N) break;  // the same for the whole warp
-        const Aux now = next;
-        if (c0 + 32 < kBN) next.load<kEpi>(a, aux, low_row, x.n0 + c0 + 32, mine);
-        uint32_t v[32];
-        __syncwarp();
+      for (int c0 = 0; c0 < cols; c0 += 64) {
+        uint32_t v[64];
         if (have) {
-          ld32(v, tmem + (static_cast<uint32_t>(32 * quarter) << 16) + static_cast<uint32_t>(b * kBN + c0));
+          ld64(v, tmem + (static_cast<uint32_t>(32 * quarter) << 16) + static_cast<uint32_t>(b * kBN + c0));
+          if (c0 + 64 >= cols) {  // read to the end: the accumulator is free
+            fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_at(bar_at<kCG>(&c.acc_empty[b], 0));
+          }
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = 0u;
+          for (int e = 0; e < 64; ++e) v[e] = 0u;
         }
-        if (!mine) continue;
+        if (rows == 0) continue;  // the whole warp
+        unsigned char* out = outs;
+        unsigned char* lows = all_lows;
+        if (kEpi == kDRelu2) {  // h lies where the result will be staged
+          if (c0 + 64 < cols) fetch(steps + 1, x.n0 + c0 + 64, row0);
+          out += (steps & 1) * kOutBytes;
+          lows += (steps & 1) * kLowBytes;
+          if (!(ok = warp_wait(&c.aux[quarter][steps & 1], static_cast<uint32_t>((steps >> 1) & 1)))) break;
+          ++steps;
+        }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = x.n0 + c0 + 8 * q;
-          if (n >= a.N) break;
-          const bf16* ah = reinterpret_cast<const bf16*>(&now.v[q]);
-          const int8_t* al = reinterpret_cast<const int8_t*>(&now.low[q / 2]) + 8 * (q % 2);
+        for (int q = 0; q < 8; ++q) {
+          uint4 av = make_uint4(0u, 0u, 0u, 0u);
+          uint2 lv = make_uint2(0u, 0u);
+          if (kEpi == kDRelu2) {
+            av = *reinterpret_cast<const uint4*>(out + out_at(lane, q));
+            if (a.low != nullptr) lv = *reinterpret_cast<const uint2*>(lows + low_at(lane, q / 2) + 8 * (q % 2));
+          }
+          const bf16* ah = reinterpret_cast<const bf16*>(&av);
+          const int8_t* al = reinterpret_cast<const int8_t*>(&lv);
           uint4 o;
-          uint2 l;
           __nv_bfloat162* oh = reinterpret_cast<__nv_bfloat162*>(&o);
-          int8_t* ol = reinterpret_cast<int8_t*>(&l);
+          uint32_t l[2] = {0u, 0u};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float h0 = 0.0f, h1 = 0.0f;
@@ -564,21 +585,40 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float y1 = finish<kEpi>(__uint_as_float(v[8 * q + 2 * e + 1]), h1, scale);
             oh[e] = __floats2bfloat162_rn(y0, y1);
             if (kEpi == kRelu2) {
-              ol[2 * e] = static_cast<int8_t>(low_bits(y0, oh[e].x));
-              ol[2 * e + 1] = static_cast<int8_t>(low_bits(y1, oh[e].y));
+              const uint32_t both = (static_cast<uint32_t>(low_bits(y0, oh[e].x)) & 255u) |
+                                    (static_cast<uint32_t>(low_bits(y1, oh[e].y)) & 255u) << 8;
+              l[e / 2] |= both << (16 * (e % 2));
             }
           }
-          *reinterpret_cast<uint4*>(out + n) = o;
-          if (kEpi == kRelu2 && a.low != nullptr) *reinterpret_cast<uint2*>(low_row + n) = l;
+          *reinterpret_cast<uint4*>(out + out_at(lane, q)) = o;
+          if (kEpi == kRelu2) *reinterpret_cast<uint2*>(lows + low_at(lane, q / 2) + 8 * (q % 2)) = make_uint2(l[0], l[1]);
         }
-      }
-      if (have) {
-        fence_before();
         __syncwarp();
-        if (lane == 0) arrive_at(bar_at<kCG>(&c.acc_empty[b], 0));
-        ++done;
+        const int n = x.n0 + c0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 4 * i + (lane >> 3), m = n + 8 * (lane & 7);
+          const int64_t dst = !kWGrad && a.scatter != nullptr ? __shfl_sync(0xffffffffu, to, r) : row0 + r;
+          if (r < rows && m < a.N)
+            *reinterpret_cast<uint4*>(a.out + dst * a.N + m) =
+                *reinterpret_cast<const uint4*>(out + out_at(r, lane & 7));
+        }
+        if (kEpi == kRelu2 && a.low != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 8 * i + (lane >> 2), m = n + 16 * (lane & 3);
+            if (r >= rows || m >= a.N) continue;
+            *reinterpret_cast<uint4*>(a.low + (row0 + r) * low_stride(a.N) + m) =
+                *reinterpret_cast<const uint4*>(lows + low_at(r, lane & 3));
+          }
+        }
+        if (kEpi == kDRelu2) fence_proxy_async();  // the next box lands here
+        __syncwarp();
       }
+      if (have) ++done;
     }
+    for (; !ok && steps < asked; ++steps)  // as above: the copies in flight end first
+      mbar_wait(&c.aux[quarter][steps & 1], static_cast<uint32_t>((steps >> 1) & 1));
     if (!kWGrad && a.zero_tail) {
       const int64_t pieces = a.N / 8;
       const int64_t end = a.R * pieces;

@@ -43,17 +43,21 @@ cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
 // has all its rows of a stage; one whose m or n is contiguous, 64 rows of k.
 template <int kCG, int kBN, bool kAMN, bool kBMN, bool kWGrad, int kEpi>
 int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2, const Args& a, cudaStream_t s) {
-  using Sh = Shape<kCG, kBN>;
+  using Sh = Shape<kCG, kBN, kEpi>;
   if (!tma::bind_context()) return camoe::tm::status(cudaErrorNoDevice);
   CUtensorMap m[4];
   const int ra = kAMN ? 64 : 128, rb = kBMN ? 64 : kBN / kCG;
   bool ok = tma::encode_3d_sw128(&m[0], A.base, A.inner, A.rows, A.depth, ra) &&
             tma::encode_3d_sw128(&m[1], B.base, B.inner, B.rows, B.depth, rb);
-  if (a.K2 > 0)
+  if (kEpi == kDRelu2)  // A2: h, B2: low, in the epilogue's boxes of 32 rows
+    ok = ok && tma::encode_3d_sw128(&m[2], A2.base, A2.inner, A2.rows, 1, 32) &&
+         (a.low == nullptr || tma::encode_2d_bytes(&m[3], a.low, low_stride(a.N), a.R, 64, 32));
+  else if (a.K2 > 0)
     ok = ok && tma::encode_3d_sw128(&m[2], A2.base, A2.inner, A2.rows, A2.depth, ra) &&
          tma::encode_3d_sw128(&m[3], B2.base, B2.inner, B2.rows, B2.depth, rb);
   else
     m[2] = m[0], m[3] = m[1];
+  if (kEpi == kDRelu2 && a.low == nullptr) m[3] = m[2];
   if (!ok) return camoe::tm::status(cudaErrorInvalidValue);
   const int64_t nt = (a.N + kBN - 1) / kBN;
   const int64_t rt = kWGrad ? static_cast<int64_t>(a.groups) * ((a.M + Sh::kBM - 1) / Sh::kBM)
@@ -64,7 +68,7 @@ int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2,
   if (nt * rt < pairs) pairs = nt * rt > 0 ? nt * rt : 1;
   const auto kernel = gemm_kernel<kCG, kBN, kAMN, kBMN, kWGrad, kEpi>;
   static std::atomic<uint64_t> opted{0};
-  constexpr int smem = smem_bytes<kCG, kBN>();
+  constexpr int smem = smem_bytes<kCG, kBN, kEpi>();
   if (const int st = camoe::tm::status(allow_smem(kernel, smem, opted))) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(pairs * kCG));

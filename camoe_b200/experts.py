@@ -173,7 +173,7 @@ def _ffn(xs, w_up, w_down, offsets, low: bool):
     R, C = xs.shape
     E, F, _ = w_up.shape
     h = torch.empty(R, F, dtype=xs.dtype, device=xs.device)
-    h_low = torch.empty(R, F, dtype=torch.int8, device=xs.device) if low else None
+    h_low = torch.empty(R, (F + 15) // 16 * 16, dtype=torch.int8, device=xs.device) if low else None
     ys = torch.empty(R, C, dtype=xs.dtype, device=xs.device)
     check(_lib.lib().camoe_ex_ffn_fwd(xs.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), offsets.data_ptr(),
                                       h.data_ptr(), None if h_low is None else h_low.data_ptr(), ys.data_ptr(), R, E, C, F,

@@ -56,8 +56,8 @@ int camoe_ex_combine_bwd(const void* dout, int dtype, const void* ys, const floa
 /* The experts' products over sorted rows, bf16: for the rows p of expert e
  *   h[p]  = relu(w_up[e] xs[p])^2      w_up   [E, F, C]
  *   ys[p] = w_down[e] h[p]             w_down [E, C, F]
- * h [R, F] is written too, and h_low [R, F] (bytes, may be NULL): the 8 bits of
- * h below bf16's, for the backward.  The rows behind offsets[E] of ys are zeros.
+ * h [R, F] is written too, and h_low [R, F rounded up to 16] (bytes, may be
+ * NULL): the 8 bits of h below bf16's, for the backward.  The rows behind offsets[E] of ys are zeros.
  * C and F are multiples of 8. */
 int camoe_ex_ffn_fwd(const void* xs, const void* w_up, const void* w_down, const int32_t* offsets,
                      void* h, void* h_low, void* ys, int64_t R, int64_t E, int64_t C, int64_t F, void* stream);
