@@ -14,9 +14,9 @@
 //     (128-byte swizzle); a piece that passes the end of a matrix reads zeros;
 //   * warp 1 issues the products, K = 16 at a time, into one of two accumulators
 //     in tensor memory, so that
-//   * warps 2-5 read the other one (an output row per thread) and write the
+//   * warps 2-9 read the other one (an output row per thread) and write the
 //     previous tile meanwhile, turned through shared memory so that a warp's
-//     stores (and its loads of h) are whole 128-byte row segments.
+//     stores are 64-byte row segments.
 // A row tile starts at its group's first row and may reach into the next
 // group's rows: those outputs are not written.  Where the sum runs over the
 // rows (weight gradients) the last piece of a group is cleared behind the
@@ -38,7 +38,8 @@ namespace camoe {
 namespace tc {
 
 constexpr int kBK = 64;           // depth of a stage: one 128-byte swizzled row of bf16
-constexpr int kThreads = 192;     // producer, product issue, four epilogue warps
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;  // producer, product issue, epilogue
 constexpr int kMaxGroups = 1025;  // 1024 and the rows of no group
 constexpr int kRingBytes = 192 * 1024;
 constexpr uint32_t kBox = 64 * 128;  // a box of 64 columns x 64 rows
@@ -67,8 +68,8 @@ struct Args {
   const int* scatter;    // output row of row p, or null
 };
 
-// Per epilogue warp: 32 rows x 64 columns of bf16, and of bytes
-constexpr uint32_t kOutBytes = 32 * 128, kLowBytes = 32 * 64;
+// Per epilogue warp: 32 rows x 32 columns of bf16, and of bytes
+constexpr uint32_t kOutBytes = 32 * 64, kLowBytes = 32 * 32;
 
 template <int kCG, int kBN, int kEpi>
 struct Shape {
@@ -77,14 +78,14 @@ struct Shape {
   static constexpr uint32_t kBBytes = kBN / kCG * 128;
   // kDRelu2 reads h a step ahead: two staging buffers per warp, in place of a stage
   static constexpr int kBufs = kEpi == kDRelu2 ? 2 : 1;
-  static constexpr int kFit = (kRingBytes - (kBufs - 1) * 32 * 1024) / (kABytes + kBBytes);
+  static constexpr int kFit = (kRingBytes - (kBufs - 1) * kEpiWarps * static_cast<int>(kOutBytes + kLowBytes)) / (kABytes + kBBytes);
   static constexpr int kStages = kFit < 10 ? kFit : 10;
-  static constexpr uint32_t kStaging = 4 * kBufs * (kOutBytes + kLowBytes);
+  static constexpr uint32_t kStaging = kEpiWarps * kBufs * (kOutBytes + kLowBytes);
   static constexpr uint32_t kCols = 2 * kBN;              // two accumulators
 };
 
 struct Control {
-  uint64_t full[10], empty[10], tail[10], peer_tail[10], acc_full[2], acc_empty[2], drained, aux[4][2];
+  uint64_t full[10], empty[10], tail[10], peer_tail[10], acc_full[2], acc_empty[2], drained, aux[kEpiWarps][2];
   uint32_t tmem;
   int tiles[kMaxGroups + 1];  // row tiles of the groups before each
 };
@@ -216,23 +217,17 @@ __device__ __forceinline__ void pair_sync() {
   else
     __syncthreads();
 }
-// 64 consecutive accumulator columns of this thread's TMEM lane (the wait is in the
+// 32 consecutive accumulator columns of this thread's TMEM lane (the wait is in the
 // same statement, so that no use of v can be moved before it)
-__device__ __forceinline__ void ld64(uint32_t (&v)[64], uint32_t taddr) {
+__device__ __forceinline__ void ld32(uint32_t (&v)[32], uint32_t taddr) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
       "tcgen05.wait::ld.sync.aligned;\n"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
         "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
         "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]),
-        "=r"(v[32]), "=r"(v[33]), "=r"(v[34]), "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]),
-        "=r"(v[40]), "=r"(v[41]), "=r"(v[42]), "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]),
-        "=r"(v[48]), "=r"(v[49]), "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]),
-        "=r"(v[56]), "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63])
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(taddr)
       : "memory");
 }
@@ -334,10 +329,11 @@ __device__ __forceinline__ float finish(float x, float aux, float scale) {
   return x;
 }
 
-// 16-byte piece q of row r in a warp's staging buffers: swizzled, so that both a
-// thread per row and eight (four) threads per row touch all banks
-__device__ __forceinline__ uint32_t out_at(int r, int q) { return r * 128 + ((q ^ (r & 7)) << 4); }
-__device__ __forceinline__ uint32_t low_at(int r, int q) { return r * 64 + ((q ^ ((r >> 1) & 3)) << 4); }
+// 16-byte piece q of row r in a warp's staging buffers: swizzled (as TMA swizzles rows
+// of 64 and of 32 bytes), so that both a thread per row and four (two) threads
+// per row touch all banks
+__device__ __forceinline__ uint32_t out_at(int r, int q) { return r * 64 + ((q ^ ((r >> 1) & 3)) << 4); }
+__device__ __forceinline__ uint32_t low_at(int r, int q) { return r * 32 + ((q ^ ((r >> 2) & 1)) << 4); }
 
 template <int kCG, int kBN, bool kAMN, bool kBMN, bool kWGrad, int kEpi>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -365,10 +361,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&c.acc_full[b], 1);
-      mbar_init(&c.acc_empty[b], 4 * kCG);
+      mbar_init(&c.acc_empty[b], kEpiWarps * kCG);
     }
     mbar_init(&c.drained, 1);
-    for (int w = 0; w < 4; ++w)
+    for (int w = 0; w < kEpiWarps; ++w)
       for (int b = 0; b < Sh::kBufs; ++b) mbar_init(&c.aux[w][b], 1);
     mbar_fence_init();
   }
@@ -506,14 +502,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3;
-    unsigned char* outs = staging + quarter * (Sh::kBufs * kOutBytes);
-    unsigned char* all_lows = staging + 4 * Sh::kBufs * kOutBytes + quarter * (Sh::kBufs * kLowBytes);
+    // two warps per 32 rows (a warp reads the tensor-memory lanes of its number mod 4), half of the columns each
+    const int quarter = warp & 3, ew = warp - 2, half = ew >> 2;
+    unsigned char* outs = staging + ew * (Sh::kBufs * kOutBytes);
+    unsigned char* all_lows = staging + kEpiWarps * Sh::kBufs * kOutBytes + ew * (Sh::kBufs * kLowBytes);
     int steps = 0, asked = 0;  // kDRelu2: boxes of h this warp has read, and asked for
-    const auto fetch = [&](int step, int n, int64_t row) {  // 64 columns of h and low
+    const auto fetch = [&](int step, int n, int64_t row) {  // 32 columns of h and low
       asked = step + 1;
       if (lane != 0) return;
-      uint64_t* bar = &c.aux[quarter][step & 1];
+      uint64_t* bar = &c.aux[ew][step & 1];
       mbar_arrive_expect_tx(bar, kOutBytes + (a.low != nullptr ? kLowBytes : 0));
       load_box<1>(sm_addr(outs + (step & 1) * kOutBytes), &ma2, n, static_cast<int>(row), 0, sm_addr(bar));
       if (a.low != nullptr)
@@ -533,36 +530,38 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float scale = kEpi == kScale && a.scale != nullptr ? a.scale[x.group] : 1.0f;
       int to = 0;  // where this lane's row goes
       if (!kWGrad && a.scatter != nullptr && lane < rows) to = a.scatter[row0 + lane];
-      if (kEpi == kDRelu2 && rows > 0) fetch(steps, x.n0, row0);
+      const int cols = a.N - x.n0 < (half + 1) * (kBN / 2) ? a.N - x.n0 : (half + 1) * (kBN / 2);
+      const int begin = half * (kBN / 2);
+      if (kEpi == kDRelu2 && rows > 0 && begin < cols) fetch(steps, x.n0 + begin, row0);
       if (have && !(ok = warp_wait(&c.acc_full[b], static_cast<uint32_t>((done / 2) & 1)))) break;
       fence_after();
-      const int cols = a.N - x.n0 < kBN ? a.N - x.n0 : kBN;
+      if (have && begin >= cols && lane == 0) arrive_at(bar_at<kCG>(&c.acc_empty[b], 0));
 #pragma unroll 1
-      for (int c0 = 0; c0 < cols; c0 += 64) {
-        uint32_t v[64];
+      for (int c0 = begin; c0 < cols; c0 += 32) {
+        uint32_t v[32];
         if (have) {
-          ld64(v, tmem + (static_cast<uint32_t>(32 * quarter) << 16) + static_cast<uint32_t>(b * kBN + c0));
-          if (c0 + 64 >= cols) {  // read to the end: the accumulator is free
+          ld32(v, tmem + (static_cast<uint32_t>(32 * quarter) << 16) + static_cast<uint32_t>(b * kBN + c0));
+          if (c0 + 32 >= cols) {  // read to the end: the accumulator is free
             fence_before();
             __syncwarp();
             if (lane == 0) arrive_at(bar_at<kCG>(&c.acc_empty[b], 0));
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < 64; ++e) v[e] = 0u;
+          for (int e = 0; e < 32; ++e) v[e] = 0u;
         }
         if (rows == 0) continue;  // the whole warp
         unsigned char* out = outs;
         unsigned char* lows = all_lows;
         if (kEpi == kDRelu2) {  // h lies where the result will be staged
-          if (c0 + 64 < cols) fetch(steps + 1, x.n0 + c0 + 64, row0);
+          if (c0 + 32 < cols) fetch(steps + 1, x.n0 + c0 + 32, row0);
           out += (steps & 1) * kOutBytes;
           lows += (steps & 1) * kLowBytes;
-          if (!(ok = warp_wait(&c.aux[quarter][steps & 1], static_cast<uint32_t>((steps >> 1) & 1)))) break;
+          if (!(ok = warp_wait(&c.aux[ew][steps & 1], static_cast<uint32_t>((steps >> 1) & 1)))) break;
           ++steps;
         }
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
+        for (int q = 0; q < 4; ++q) {
           uint4 av = make_uint4(0u, 0u, 0u, 0u);
           uint2 lv = make_uint2(0u, 0u);
           if (kEpi == kDRelu2) {
@@ -596,20 +595,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         const int n = x.n0 + c0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = 4 * i + (lane >> 3), m = n + 8 * (lane & 7);
+        for (int i = 0; i < 4; ++i) {
+          const int r = 8 * i + (lane >> 2), m = n + 8 * (lane & 3);
           const int64_t dst = !kWGrad && a.scatter != nullptr ? __shfl_sync(0xffffffffu, to, r) : row0 + r;
           if (r < rows && m < a.N)
             *reinterpret_cast<uint4*>(a.out + dst * a.N + m) =
-                *reinterpret_cast<const uint4*>(out + out_at(r, lane & 7));
+                *reinterpret_cast<const uint4*>(out + out_at(r, lane & 3));
         }
         if (kEpi == kRelu2 && a.low != nullptr) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 8 * i + (lane >> 2), m = n + 16 * (lane & 3);
+          for (int i = 0; i < 2; ++i) {
+            const int r = 16 * i + (lane >> 1), m = n + 16 * (lane & 1);
             if (r >= rows || m >= a.N) continue;
             *reinterpret_cast<uint4*>(a.low + (row0 + r) * low_stride(a.N) + m) =
-                *reinterpret_cast<const uint4*>(lows + low_at(r, lane & 3));
+                *reinterpret_cast<const uint4*>(lows + low_at(r, lane & 1));
           }
         }
         if (kEpi == kDRelu2) fence_proxy_async();  // the next box lands here
@@ -618,13 +617,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (have) ++done;
     }
     for (; !ok && steps < asked; ++steps)  // as above: the copies in flight end first
-      mbar_wait(&c.aux[quarter][steps & 1], static_cast<uint32_t>((steps >> 1) & 1));
+      mbar_wait(&c.aux[ew][steps & 1], static_cast<uint32_t>((steps >> 1) & 1));
     if (!kWGrad && a.zero_tail) {
       const int64_t pieces = a.N / 8;
       const int64_t end = a.R * pieces;
       uint4* out = reinterpret_cast<uint4*>(a.out);
-      const int64_t step = static_cast<int64_t>(gridDim.x) * 128;
-      for (int64_t i = tiles.first(a.groups) * pieces + static_cast<int64_t>(blockIdx.x) * 128 + (tid - 64); i < end;
+      const int64_t step = static_cast<int64_t>(gridDim.x) * (32 * kEpiWarps);
+      for (int64_t i = tiles.first(a.groups) * pieces + static_cast<int64_t>(blockIdx.x) * (32 * kEpiWarps) + (tid - 64); i < end;
            i += step)
         out[i] = make_uint4(0u, 0u, 0u, 0u);
     }

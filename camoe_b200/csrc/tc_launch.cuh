@@ -50,8 +50,8 @@ int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2,
   bool ok = tma::encode_3d_sw128(&m[0], A.base, A.inner, A.rows, A.depth, ra) &&
             tma::encode_3d_sw128(&m[1], B.base, B.inner, B.rows, B.depth, rb);
   if (kEpi == kDRelu2)  // A2: h, B2: low, in the epilogue's boxes of 32 rows
-    ok = ok && tma::encode_3d_sw128(&m[2], A2.base, A2.inner, A2.rows, 1, 32) &&
-         (a.low == nullptr || tma::encode_2d_bytes(&m[3], a.low, low_stride(a.N), a.R, 64, 32));
+    ok = ok && tma::encode_2d_rows(&m[2], A2.base, 2 * A2.inner, A2.rows, 64, 32) &&
+         (a.low == nullptr || tma::encode_2d_rows(&m[3], a.low, low_stride(a.N), a.R, 32, 32));
   else if (a.K2 > 0)
     ok = ok && tma::encode_3d_sw128(&m[2], A2.base, A2.inner, A2.rows, A2.depth, ra) &&
          tma::encode_3d_sw128(&m[3], B2.base, B2.inner, B2.rows, B2.depth, rb);

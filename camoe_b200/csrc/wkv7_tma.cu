@@ -83,21 +83,25 @@ bool encode_3d_sw128(CUtensorMap* map, const void* base, int64_t inner, int64_t 
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool encode_2d_bytes(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int box_inner,
-                     int box_rows) {
+bool encode_2d_rows(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t rows, int box_bytes,
+                    int box_rows) {
   const EncodeFn fn = encode_fn();
-  if (fn == nullptr || inner <= 0 || rows <= 0 || inner % 16 != 0 || box_inner != 64 || box_rows <= 0 ||
-      box_rows > 256)
+  if (fn == nullptr || row_bytes <= 0 || rows <= 0 || row_bytes % 16 != 0 ||
+      (box_bytes != 32 && box_bytes != 64) || box_rows <= 0 || box_rows > 256)
     return false;
-  // a third dimension of one, so that it is loaded like the other maps
-  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows), 1};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(inner),
-                                 static_cast<cuuint64_t>(inner) * static_cast<cuuint64_t>(rows)};
-  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_rows), 1};
+  // bf16 where the box holds 32 columns of it, bytes otherwise; a third dimension
+  // of one, so that it is loaded like the other maps
+  const bool two = box_bytes == 64;
+  const cuuint64_t size = two ? 2 : 1;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(row_bytes) / size, static_cast<cuuint64_t>(rows), 1};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_bytes),
+                                 static_cast<cuuint64_t>(row_bytes) * static_cast<cuuint64_t>(rows)};
+  const cuuint32_t box[3] = {32, static_cast<cuuint32_t>(box_rows), 1};
   const cuuint32_t estride[3] = {1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estride,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return fn(map, two ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3,
+            const_cast<void*>(base), dims, strides, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            two ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 bool encode_bhtn_f32(CUtensorMap* map, const void* base, int64_t B, int64_t T, int64_t H) {

@@ -56,11 +56,12 @@ bool encode_2d_sw128(CUtensorMap* map, const void* base, int64_t inner, int64_t 
 bool encode_3d_sw128(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int64_t depth,
                      int box_rows);
 
-// Map of a row-major byte matrix [rows][inner] (inner a multiple of 16) with boxes of
-// box_inner = 64 bytes x box_rows and the 64-byte swizzle (16-byte piece q of row
-// r lands at piece q ^ ((r >> 1) & 3)).
-bool encode_2d_bytes(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int box_inner,
-                     int box_rows);
+// Map of a row-major matrix of `row_bytes` (a multiple of 16) per row with boxes of 32
+// columns x box_rows: box_bytes 64 for bf16 with the 64-byte swizzle (16-byte
+// piece q of row r lands at piece q ^ ((r >> 1) & 3)), 32 for bytes with the
+// 32-byte one (q ^ ((r >> 2) & 1)).
+bool encode_2d_rows(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t rows, int box_bytes,
+                    int box_rows);
 
 // Load the box at (x, y, z) of a 3-D map, completing on `bar`.
 __device__ __forceinline__ void load_3d(void* dst_smem, const CUtensorMap* map, int x, int y, int z,
