@@ -4,8 +4,9 @@
 //
 // Few rows (a token of each of many requests): two launches.  low[n] = scale[a]
 // down[a] x[n] in fp32, a warp per output; then the projection with the weights
-// streamed once (rows_mma.cuh), to whose sums each output adds its row of up
-// times low, in fp32, before the one rounding.
+// streamed once (tc_thin.cuh; it starts while the first kernel runs), to whose
+// sums each output adds its row of up times low, in fp32, before the one
+// rounding.
 //
 // Many rows (prompts): the rows are sorted by adapter, low = scale (xs down^T)
 // is one grouped product (rounded to bf16, the type of the next product's
@@ -14,7 +15,6 @@
 // columns of K in the tensor cores, its bytes are read once per row tile, and
 // the result goes to the row that it came from.
 #include "camoe_experts.h"
-#include "rows_mma.cuh"
 #include "tc_launch.cuh"
 
 namespace camoe {
@@ -40,6 +40,7 @@ __global__ void __launch_bounds__(kThreads) low_kernel(const bf16* __restrict__ 
                                                        const int* __restrict__ adapter,
                                                        const float* __restrict__ scale,
                                                        float* __restrict__ low, int C, int D, int L) {
+  thin::allow_next();
   const int n = blockIdx.y, lane = threadIdx.x & 31;
   const int d = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   const int a = adapter[n];
@@ -48,7 +49,7 @@ __global__ void __launch_bounds__(kThreads) low_kernel(const bf16* __restrict__ 
   const bf16* dp = down + (static_cast<int64_t>(a) * D + d) * C;
   float s = 0.0f;
   for (int v = lane; v < C / 8; v += 32) {
-    const uint4 p = xp[v], q = thin::ld_once(dp + 8 * v);
+    const uint4 p = xp[v], q = *reinterpret_cast<const uint4*>(dp + 8 * v);
     const __nv_bfloat162* ph = reinterpret_cast<const __nv_bfloat162*>(&p);
     const __nv_bfloat162* qh = reinterpret_cast<const __nv_bfloat162*>(&q);
 #pragma unroll
@@ -61,49 +62,6 @@ __global__ void __launch_bounds__(kThreads) low_kernel(const bf16* __restrict__ 
 #pragma unroll
   for (int m = 16; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
   if (lane == 0) low[static_cast<int64_t>(n) * D + d] = scale != nullptr ? scale[a] * s : s;
-}
-
-template <int kN>
-__global__ void __launch_bounds__(thin::kThreads) thin_kernel(const bf16* __restrict__ x,
-                                                              const bf16* __restrict__ w,
-                                                              const bf16* __restrict__ up,
-                                                              const int* __restrict__ adapter,
-                                                              const float* __restrict__ low,
-                                                              bf16* __restrict__ y, int64_t N, int C, int M, int D,
-                                                              int L) {
-  __shared__ __align__(16) float red[thin::kWarps * thin::kO * 8 * kN];
-  const int o0 = blockIdx.x * thin::kO, n_o = M - o0 < thin::kO ? M - o0 : thin::kO;
-  const int64_t p = static_cast<int64_t>(blockIdx.y) * 8 * kN;
-  const int n_r = N - p < 8 * kN ? static_cast<int>(N - p) : 8 * kN;
-  thin::block_sums<kN>(w + static_cast<int64_t>(o0) * C, n_o, x + p * C, n_r, C, red);
-  for (int i = threadIdx.x; i < thin::kO * 8 * kN; i += thin::kThreads) {
-    const int o = i % thin::kO, r = i / thin::kO;
-    if (o >= n_o || r >= n_r) continue;
-    float v = thin::total<kN>(red, o, r);
-    const int a = adapter[p + r];
-    if (a >= 0 && a < L) {
-      const uint4* u = reinterpret_cast<const uint4*>(up + (static_cast<int64_t>(a) * M + o0 + o) * D);
-      const float4* l = reinterpret_cast<const float4*>(low + (p + r) * D);
-      float s = 0.0f;
-      for (int d = 0; d < D / 8; ++d) {
-        const uint4 q = u[d];
-        const float4 l0 = l[2 * d], l1 = l[2 * d + 1];
-        const __nv_bfloat162* qh = reinterpret_cast<const __nv_bfloat162*>(&q);
-        const float2 q0 = __bfloat1622float2(qh[0]), q1 = __bfloat1622float2(qh[1]),
-                     q2 = __bfloat1622float2(qh[2]), q3 = __bfloat1622float2(qh[3]);
-        s = fmaf(q0.x, l0.x, s);
-        s = fmaf(q0.y, l0.y, s);
-        s = fmaf(q1.x, l0.z, s);
-        s = fmaf(q1.y, l0.w, s);
-        s = fmaf(q2.x, l1.x, s);
-        s = fmaf(q2.y, l1.y, s);
-        s = fmaf(q3.x, l1.z, s);
-        s = fmaf(q3.y, l1.w, s);
-      }
-      v += s;
-    }
-    y[(p + r) * M + o0 + o] = __float2bfloat16_rn(v);
-  }
 }
 
 // Rows that are streamed rather than sorted: a few, or so few per adapter that
@@ -184,16 +142,22 @@ int camoe_ad_linear(const void* x, const void* weight, const void* down, const v
       low_kernel<<<dim3((d + 7) / 8, static_cast<unsigned>(n)), kThreads, 0, s>>>(
           xb + n0 * C, static_cast<const bf16*>(down), adapter + n0, scale, low + n0 * D, c, d, l);
     }
-    const unsigned gx = static_cast<unsigned>((M + thin::kO - 1) / thin::kO);
-    if (N <= 8)
-      thin_kernel<1><<<dim3(gx, 1), thin::kThreads, 0, s>>>(xb, static_cast<const bf16*>(weight),
-                                                            static_cast<const bf16*>(up), adapter, low,
-                                                            static_cast<bf16*>(y), N, c, m, d, l);
-    else
-      thin_kernel<4><<<dim3(gx, static_cast<unsigned>((N + 31) / 32)), thin::kThreads, 0, s>>>(
-          xb, static_cast<const bf16*>(weight), static_cast<const bf16*>(up), adapter, low,
-          static_cast<bf16*>(y), N, c, m, d, l);
-    return camoe::tm::status(cudaGetLastError());
+    thin::Args t{};
+    t.groups = 1;
+    t.R = N;
+    t.O = m;
+    t.K = c;
+    t.out = static_cast<bf16*>(y);
+    t.up = static_cast<const bf16*>(up);
+    t.adapter = adapter;
+    t.low_rank = low;
+    t.D = d;
+    t.L = l;
+    if (const int st = camoe::tm::status(cudaGetLastError())) return st;
+    if (N <= 16) return thin::launch<16, thin::kAdapter>(x, weight, t, 1, 1, true, s);
+    if (N <= 32) return thin::launch<32, thin::kAdapter>(x, weight, t, 1, 1, true, s);
+    if (N <= 64) return thin::launch<64, thin::kAdapter>(x, weight, t, 1, 1, true, s);
+    return thin::launch<128, thin::kAdapter>(x, weight, t, 1, (N + 127) / 128, true, s);
   }
   bf16* low = reinterpret_cast<bf16*>(base + w.low);
   bf16* xs = reinterpret_cast<bf16*>(base + w.xs);

@@ -14,7 +14,6 @@
 // its rounding error to dpre's own (2.5e-3 against 2.4e-3 of dxs and dw_up in the
 // 2-norm, where one rounding is 1.7e-3).
 #include "camoe_experts.h"
-#include "rows_mma.cuh"
 #include "tc_gemm.cuh"
 #include "tc_launch.cuh"
 
@@ -31,86 +30,29 @@ unsigned int ffn_timeouts() {
 
 namespace ffn {
 
-// The y-th group that has rows; false where there are fewer.
-__device__ __forceinline__ bool nth_group(const int* offsets, int E, int64_t R, int y, int* g, int64_t* r0,
-                                          int64_t* r1) {
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int e0 = 0; e0 < E; e0 += 32) {
-    const int e = e0 + lane;
-    int64_t a = 0, b = 0;
-    if (e < E) {
-      a = offsets[e];
-      b = offsets[e + 1];
-      a = a < 0 ? 0 : (a < R ? a : R);
-      b = b < 0 ? 0 : (b < R ? b : R);
-    }
-    unsigned has = __ballot_sync(0xffffffffu, b > a);
-    const int n = __popc(has);
-    if (y < before + n) {
-      for (int i = before; i < y; ++i) has &= has - 1;
-      const int src = __ffs(has) - 1;
-      *g = e0 + src;
-      *r0 = __shfl_sync(0xffffffffu, a, src);
-      *r1 = __shfl_sync(0xffffffffu, b, src);
-      return true;
-    }
-    before += n;
-  }
-  return false;
-}
+// Few rows per expert: the weights' bytes decide, and tiles of a few rows read them
+// at HBM rate; with more the products count, and 256-row tiles are faster.
+bool few_rows(int64_t R, int64_t E) { return R <= 64 * E; }
 
-// out[p][o] = f(sum over k x[p][k] w[e][o][k]) for 16 of the O outputs of the
-// blockIdx.y-th expert that has rows, 8 kN rows at a time.
-template <int kN, bool kRelu2>
-__global__ void __launch_bounds__(thin::kThreads) thin_kernel(const bf16* __restrict__ x,
-                                                              const bf16* __restrict__ w,
-                                                              const int* __restrict__ offsets,
-                                                              bf16* __restrict__ out, int8_t* __restrict__ low,
-                                                              int64_t R, int E, int O, int K, int zero_tail) {
-  __shared__ __align__(16) float red[thin::kWarps * thin::kO * 8 * kN];
-  if (zero_tail && blockIdx.y == 0) {
-    const int64_t used = offsets[E] > 0 ? offsets[E] : 0;
-    for (int64_t i = used * O + static_cast<int64_t>(blockIdx.x) * thin::kThreads + threadIdx.x; i < R * O;
-         i += static_cast<int64_t>(gridDim.x) * thin::kThreads)
-      out[i] = __float2bfloat16_rn(0.0f);
-  }
-  int e;
-  int64_t r0, r1;
-  if (!nth_group(offsets, E, R, blockIdx.y, &e, &r0, &r1)) return;
-  const int o0 = blockIdx.x * thin::kO, n_o = O - o0 < thin::kO ? O - o0 : thin::kO;
-  const bf16* we = w + (static_cast<int64_t>(e) * O + o0) * K;
-  for (int64_t p = r0; p < r1; p += 8 * kN) {
-    const int n_r = r1 - p < 8 * kN ? static_cast<int>(r1 - p) : 8 * kN;
-    thin::block_sums<kN>(we, n_o, x + p * K, n_r, K, red);
-    for (int i = threadIdx.x; i < thin::kO * 8 * kN; i += thin::kThreads) {
-      const int o = i % thin::kO, r = i / thin::kO;
-      if (o < n_o && r < n_r) {
-        float v = thin::total<kN>(red, o, r);
-        if (kRelu2) v = v < 0.0f ? 0.0f : v * v;
-        const bf16 hi = __float2bfloat16_rn(v);
-        out[(p + r) * O + o0 + o] = hi;
-        if (kRelu2 && low != nullptr) low[(p + r) * tc::low_stride(O) + o0 + o] = static_cast<int8_t>(tc::low_bits(v, hi));
-      }
-    }
-    __syncthreads();  // red is written again
-  }
-}
-
-// Few rows per expert: the weights' bytes decide, and the streaming kernel reads
-// them at HBM rate; with more rows than that the tensor memory kernel is faster.
-bool few_rows(int64_t R, int64_t E) { return R <= 16 * E && R <= 512; }
-
-template <bool kRelu2>
+// kN: rows of an expert that go through a tile at once; twice the mean of the
+// experts' rows, so that most experts' weights are read once.
+template <int kEpi>
 int thin_product(const bf16* x, const bf16* w, const int* offsets, bf16* out, int8_t* low, int64_t R, int64_t E,
-                 int64_t O, int64_t K, bool zero_tail, cudaStream_t st) {
-  const dim3 g(static_cast<unsigned>((O + thin::kO - 1) / thin::kO), static_cast<unsigned>(E < R ? E : R));
-  const int e = static_cast<int>(E), o = static_cast<int>(O), k = static_cast<int>(K);
-  if (R <= 2 * E)
-    thin_kernel<1, kRelu2><<<g, thin::kThreads, 0, st>>>(x, w, offsets, out, low, R, e, o, k, zero_tail);
-  else
-    thin_kernel<4, kRelu2><<<g, thin::kThreads, 0, st>>>(x, w, offsets, out, low, R, e, o, k, zero_tail);
-  return camoe::tm::status(cudaGetLastError());
+                 int64_t O, int64_t K, bool second, cudaStream_t st) {
+  thin::Args a{};
+  a.offsets = offsets;
+  a.groups = static_cast<int>(E);
+  a.R = R;
+  a.O = static_cast<int>(O);
+  a.K = static_cast<int>(K);
+  a.x_waits = a.zero_tail = second ? 1 : 0;
+  a.out = out;
+  a.low = low;
+  const int64_t groups = E < R ? E : R;
+  if (R <= 8 * E) return thin::launch<16, kEpi>(x, w, a, groups, 1, second, st);
+  if (R <= 16 * E) return thin::launch<32, kEpi>(x, w, a, groups, 1, second, st);
+  if (R <= 32 * E) return thin::launch<64, kEpi>(x, w, a, groups, 1, second, st);
+  return thin::launch<128, kEpi>(x, w, a, groups, 1, second, st);
 }
 
 tc::Args args(const int* offsets, int64_t E, int64_t R, int64_t N, int64_t K, void* out) {
@@ -163,10 +105,10 @@ int camoe_ex_ffn_fwd(const void* xs, const void* w_up, const void* w_down, const
   int8_t* low = static_cast<int8_t*>(h_low);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (few_rows(R, E)) {
-    const int st = thin_product<true>(static_cast<const bf16*>(xs), static_cast<const bf16*>(w_up), offsets,
+    const int st = thin_product<tc::kRelu2>(static_cast<const bf16*>(xs), static_cast<const bf16*>(w_up), offsets,
                                       static_cast<bf16*>(h), low, R, E, F, C, false, s);
     if (st != 0) return st;
-    return thin_product<false>(static_cast<const bf16*>(h), static_cast<const bf16*>(w_down), offsets,
+    return thin_product<tc::kPlain>(static_cast<const bf16*>(h), static_cast<const bf16*>(w_down), offsets,
                                static_cast<bf16*>(ys), nullptr, R, E, C, F, true, s);
   }
   tc::Args up = args(offsets, E, R, F, C, h);

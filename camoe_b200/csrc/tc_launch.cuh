@@ -4,6 +4,7 @@
 #include <atomic>
 
 #include "tc_gemm.cuh"
+#include "tc_thin.cuh"
 
 namespace camoe {
 namespace tm {
@@ -85,4 +86,48 @@ int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2,
 }
 
 }  // namespace tc
+
+namespace thin {
+
+// CTAs per tile of 128 outputs: as many as keep all of them on the SMs at once (two
+// per SM up to kN = 64), with two pieces of k at least for each
+inline int split_of(int64_t tiles, int64_t K, int per_sm) {
+  const int64_t nk = (K + tc::kBK - 1) / tc::kBK, room = per_sm * tc::sm_count();
+  int s = 1;
+  while (s < 8 && tiles * s * 2 <= room && nk >= 4 * s) s *= 2;
+  return s;
+}
+
+// `groups` that can have rows, `row_tiles` started apart (1: one after the other);
+// `early`: may start before the kernel before it in the stream has ended.
+template <int kN, int kEpi>
+int launch(const void* x, const void* w, Args a, int64_t groups, int64_t row_tiles, bool early, cudaStream_t s) {
+  if (!tma::bind_context()) return camoe::tm::status(cudaErrorNoDevice);
+  CUtensorMap mw, mx;
+  if (!tma::encode_3d_sw128(&mw, w, a.K, a.O, a.groups, kM) || !tma::encode_3d_sw128(&mx, x, a.K, a.R, 1, kN))
+    return camoe::tm::status(cudaErrorInvalidValue);
+  const int64_t tiles = (a.O + kM - 1) / kM;
+  a.split = split_of(tiles * groups * row_tiles, a.K, kN <= 64 ? 2 : 1);
+  const auto kernel = thin_kernel<kN, kEpi>;
+  static std::atomic<uint64_t> opted{0};
+  constexpr int smem = smem_bytes<kN>();
+  if (const int st = camoe::tm::status(tc::allow_smem(kernel, smem, opted))) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * a.split), static_cast<unsigned>(groups),
+                     static_cast<unsigned>(row_tiles));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(a.split);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 2 : 1;
+  return camoe::tm::status(cudaLaunchKernelEx(&cfg, kernel, mw, mx, a));
+}
+
+}  // namespace thin
 }  // namespace camoe
