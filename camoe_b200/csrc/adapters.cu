@@ -154,10 +154,11 @@ int camoe_ad_linear(const void* x, const void* weight, const void* down, const v
     t.D = d;
     t.L = l;
     if (const int st = camoe::tm::status(cudaGetLastError())) return st;
-    if (N <= 16) return thin::launch<16, thin::kAdapter>(x, weight, t, 1, 1, true, s);
-    if (N <= 32) return thin::launch<32, thin::kAdapter>(x, weight, t, 1, 1, true, s);
-    if (N <= 64) return thin::launch<64, thin::kAdapter>(x, weight, t, 1, 1, true, s);
-    return thin::launch<128, thin::kAdapter>(x, weight, t, 1, (N + 127) / 128, true, s);
+    t.second = 1;
+    // row tiles of 32 started apart: their adapters' work runs side by side, and
+    // the weights of all but one come from L2
+    return N <= 16 ? thin::launch<16, thin::kAdapter>(x, weight, t, 1, 1, s)
+                   : thin::launch<32, thin::kAdapter>(x, weight, t, 1, (N + 31) / 32, s);
   }
   bf16* low = reinterpret_cast<bf16*>(base + w.low);
   bf16* xs = reinterpret_cast<bf16*>(base + w.xs);

@@ -45,14 +45,14 @@ int thin_product(const bf16* x, const bf16* w, const int* offsets, bf16* out, in
   a.R = R;
   a.O = static_cast<int>(O);
   a.K = static_cast<int>(K);
-  a.x_waits = a.zero_tail = second ? 1 : 0;
+  a.second = a.zero_tail = second ? 1 : 0;
   a.out = out;
   a.low = low;
   const int64_t groups = E < R ? E : R;
-  if (R <= 8 * E) return thin::launch<16, kEpi>(x, w, a, groups, 1, second, st);
-  if (R <= 16 * E) return thin::launch<32, kEpi>(x, w, a, groups, 1, second, st);
-  if (R <= 32 * E) return thin::launch<64, kEpi>(x, w, a, groups, 1, second, st);
-  return thin::launch<128, kEpi>(x, w, a, groups, 1, second, st);
+  if (R <= 8 * E) return thin::launch<16, kEpi>(x, w, a, groups, 1, st);
+  if (R <= 16 * E) return thin::launch<32, kEpi>(x, w, a, groups, 1, st);
+  if (R <= 32 * E) return thin::launch<64, kEpi>(x, w, a, groups, 1, st);
+  return thin::launch<128, kEpi>(x, w, a, groups, 1, st);
 }
 
 tc::Args args(const int* offsets, int64_t E, int64_t R, int64_t N, int64_t K, void* out) {

@@ -91,23 +91,25 @@ namespace thin {
 
 // CTAs per tile of 128 outputs: as many as keep all of them on the SMs at once (two
 // per SM up to kN = 64), with two pieces of k at least for each
-inline int split_of(int64_t tiles, int64_t K, int per_sm) {
+inline int split_of(int64_t tiles, int64_t K, int per_sm, int least) {
   const int64_t nk = (K + tc::kBK - 1) / tc::kBK, room = per_sm * tc::sm_count();
-  int s = 1;
+  int s = least;
   while (s < 8 && tiles * s * 2 <= room && nk >= 4 * s) s *= 2;
   return s;
 }
 
 // `groups` that can have rows, `row_tiles` started apart (1: one after the other);
-// `early`: may start before the kernel before it in the stream has ended.
+// The kernel may start before the one before it in the stream has ended: it waits
+// for that one before it reads what that one may have written, and in every case
+// before it ends.
 template <int kN, int kEpi>
-int launch(const void* x, const void* w, Args a, int64_t groups, int64_t row_tiles, bool early, cudaStream_t s) {
+int launch(const void* x, const void* w, Args a, int64_t groups, int64_t row_tiles, cudaStream_t s) {
   if (!tma::bind_context()) return camoe::tm::status(cudaErrorNoDevice);
   CUtensorMap mw, mx;
   if (!tma::encode_3d_sw128(&mw, w, a.K, a.O, a.groups, kM) || !tma::encode_3d_sw128(&mx, x, a.K, a.R, 1, kN))
     return camoe::tm::status(cudaErrorInvalidValue);
   const int64_t tiles = (a.O + kM - 1) / kM;
-  a.split = split_of(tiles * groups * row_tiles, a.K, kN <= 64 ? 2 : 1);
+  a.split = split_of(tiles * groups * row_tiles, a.K, kN <= 64 ? 2 : 1, kEpi == kAdapter ? kN / kAdd : 1);
   const auto kernel = thin_kernel<kN, kEpi>;
   static std::atomic<uint64_t> opted{0};
   constexpr int smem = smem_bytes<kN>();
@@ -125,7 +127,7 @@ int launch(const void* x, const void* w, Args a, int64_t groups, int64_t row_til
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = early ? 2 : 1;
+  cfg.numAttrs = 2;
   return camoe::tm::status(cudaLaunchKernelEx(&cfg, kernel, mw, mx, a));
 }
 

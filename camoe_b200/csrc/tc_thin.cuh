@@ -34,7 +34,7 @@ struct Args {
   int64_t R;
   int O, K;
   int split;           // CTAs per tile (the cluster's size)
-  int x_waits;         // x is written by the kernel before this one
+  int second;          // offsets and weights are older than the kernel before this one, x is not
   int zero_tail;       // write zeros to the rows behind the last group
   bf16* out;
   int8_t* low;         // tc::kRelu2: as in tc_gemm.cuh, or null
@@ -115,37 +115,60 @@ __device__ __forceinline__ bool nth_group(const Args& a, int y, int* g, int64_t*
 // f, and the store of output o of row p
 template <int kEpi>
 __device__ __forceinline__ void put(const Args& a, int64_t p, int o, float v) {
-  if (kEpi == kAdapter) {
-    const int ad = a.adapter[p];
-    if (ad >= 0 && ad < a.L) {
-      const uint4* u = reinterpret_cast<const uint4*>(a.up + (static_cast<int64_t>(ad) * a.O + o) * a.D);
-      const float4* l = reinterpret_cast<const float4*>(a.low_rank + p * a.D);
-      float s = 0.0f;
-#pragma unroll 4
-      for (int d = 0; d < a.D / 8; ++d) {
-        const uint4 q = u[d];
-        const float4 l0 = l[2 * d], l1 = l[2 * d + 1];
-        const __nv_bfloat162* qh = reinterpret_cast<const __nv_bfloat162*>(&q);
-        const float2 q0 = __bfloat1622float2(qh[0]), q1 = __bfloat1622float2(qh[1]),
-                     q2 = __bfloat1622float2(qh[2]), q3 = __bfloat1622float2(qh[3]);
-        s = fmaf(q0.x, l0.x, s);
-        s = fmaf(q0.y, l0.y, s);
-        s = fmaf(q1.x, l0.z, s);
-        s = fmaf(q1.y, l0.w, s);
-        s = fmaf(q2.x, l1.x, s);
-        s = fmaf(q2.y, l1.y, s);
-        s = fmaf(q3.x, l1.z, s);
-        s = fmaf(q3.y, l1.w, s);
-      }
-      v += s;
-    }
-  } else {
-    v = tc::finish<kEpi>(v, 0.0f, 1.0f);
-  }
+  if (kEpi != kAdapter) v = tc::finish<kEpi>(v, 0.0f, 1.0f);
   const bf16 hi = __float2bfloat16_rn(v);
   a.out[p * a.O + o] = hi;
   if (kEpi == tc::kRelu2 && a.low != nullptr)
     a.low[p * tc::low_stride(a.O) + o] = static_cast<int8_t>(tc::low_bits(v, hi));
+}
+
+// kAdapter: what the adapters add to output o of up to kAdd rows p, p + step, ...
+// below end; four rows at a time, so that their loads overlap.
+constexpr int kAdd = 16;
+__device__ __forceinline__ void adapter_add(const Args& a, int64_t p, int step, int64_t end, int o, float (&add)[kAdd]) {
+#pragma unroll
+  for (int r = 0; r < kAdd; r += 4) {
+    const uint4* u[4];
+    const float4* l[4];
+    bool has[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t q = p + static_cast<int64_t>(step) * (r + j);
+      const int ad = q < end && o < a.O ? a.adapter[q] : -1;
+      has[j] = ad >= 0 && ad < a.L;
+      u[j] = reinterpret_cast<const uint4*>(a.up + (static_cast<int64_t>(has[j] ? ad : 0) * a.O + o) * a.D);
+      l[j] = reinterpret_cast<const float4*>(a.low_rank + q * a.D);
+      add[r + j] = 0.0f;
+    }
+    for (int d = 0; d < a.D / 8; ++d) {
+      uint4 w[4];
+      float4 l0[4], l1[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!has[j]) continue;
+        w[j] = u[j][d];
+        l0[j] = l[j][2 * d];
+        l1[j] = l[j][2 * d + 1];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!has[j]) continue;
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w[j]);
+        const float2 q0 = __bfloat1622float2(h[0]), q1 = __bfloat1622float2(h[1]), q2 = __bfloat1622float2(h[2]),
+                     q3 = __bfloat1622float2(h[3]);
+        float s = add[r + j];
+        s = fmaf(q0.x, l0[j].x, s);
+        s = fmaf(q0.y, l0[j].y, s);
+        s = fmaf(q1.x, l0[j].z, s);
+        s = fmaf(q1.y, l0[j].w, s);
+        s = fmaf(q2.x, l1[j].x, s);
+        s = fmaf(q2.y, l1[j].y, s);
+        s = fmaf(q3.x, l1[j].z, s);
+        s = fmaf(q3.y, l1[j].w, s);
+        add[r + j] = s;
+      }
+    }
+  }
 }
 
 template <int kN>
@@ -174,6 +197,17 @@ __global__ void __launch_bounds__(kThreads) thin_kernel(const __grid_constant__ 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = a.split, rank = static_cast<int>(blockIdx.x) % split, tile = static_cast<int>(blockIdx.x) / split;
   allow_next();
+  if (tid == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mw)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mx)) : "memory");
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&c.full[s], 1);
+      mbar_init(&c.empty[s], 1);
+    }
+    mbar_init(&c.acc, 1);
+    mbar_fence_init();
+  }
+  if (!a.second) wait_previous();
   if (a.zero_tail && blockIdx.y == 0) {
     const int64_t pieces = a.O / 8, used = a.offsets != nullptr ? a.offsets[a.groups] : a.R;
     uint4* out = reinterpret_cast<uint4*>(a.out);
@@ -184,19 +218,11 @@ __global__ void __launch_bounds__(kThreads) thin_kernel(const __grid_constant__ 
   int g;
   int64_t r0, r1;
   if (!nth_group(a, static_cast<int>(blockIdx.y), &g, &r0, &r1)) {  // the whole cluster
-    if (a.x_waits) wait_previous();
+    if (a.second) wait_previous();
     return;
   }
   const int nk = (a.K + tc::kBK - 1) / tc::kBK, per = (nk + split - 1) / split;
   const int k0 = rank * per < nk ? rank * per : nk, k1 = k0 + per < nk ? k0 + per : nk;
-  if (tid == 0) {
-    for (int s = 0; s < S; ++s) {
-      mbar_init(&c.full[s], 1);
-      mbar_init(&c.empty[s], 1);
-    }
-    mbar_init(&c.acc, 1);
-    mbar_fence_init();
-  }
   if (warp == 1) tc::tmem_alloc<1>(&c.tmem, Sh::kCols);
   tc::fence_before();
   __syncthreads();
@@ -205,6 +231,7 @@ __global__ void __launch_bounds__(kThreads) thin_kernel(const __grid_constant__ 
   const int64_t start = r0 + static_cast<int64_t>(blockIdx.z) * kN, step = static_cast<int64_t>(gridDim.z) * kN;
   const int o = tile * kM + 32 * (warp & 3) + lane;
   int i = 0, it = 0;  // pieces and row tiles so far
+  float add[kAdd];    // kAdapter: kN / split rows at most, which the launch sees to
   bool ok = true;
   for (int64_t p = start; p < r1; p += step, ++it) {
     if (warp == 0) {
@@ -221,7 +248,7 @@ __global__ void __launch_bounds__(kThreads) thin_kernel(const __grid_constant__ 
         if (it == 0) {  // the first pieces' weights do not wait for x
           const int first = k1 - k0 < S ? k1 - k0 : S;
           for (int j = 0; j < first; ++j) load_w(j, k0 + j);
-          if (a.x_waits) wait_previous();
+          if (a.second) wait_previous();
           for (int j = 0; j < first; ++j) load_x(j, k0 + j);
           k += first;
           i = first;
@@ -255,9 +282,12 @@ __global__ void __launch_bounds__(kThreads) thin_kernel(const __grid_constant__ 
     }
     const int rows = r1 - p < kN ? static_cast<int>(r1 - p) : kN;
     if (warp >= 2) {
+      if (kEpi == kAdapter) {  // while the weights arrive
+        wait_previous();       // low_rank
+        adapter_add(a, p + rank, split, r1 < p + kN ? r1 : p + kN, o, add);
+      }
       if (k1 > k0) ok = tc::warp_wait(&c.acc, static_cast<uint32_t>(it & 1)) && ok;
       tc::fence_after();
-      if (kEpi == kAdapter) wait_previous();  // low_rank
       float* part = reinterpret_cast<float*>(ring) + (32 * (warp & 3) + lane);
 #pragma unroll 1
       for (int c0 = 0; c0 < kN; c0 += 16) {
@@ -273,7 +303,7 @@ __global__ void __launch_bounds__(kThreads) thin_kernel(const __grid_constant__ 
           if (o < a.O) {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              if (c0 + e < rows) put<kEpi>(a, p + c0 + e, o, v[e]);
+              if (c0 + e < rows) put<kEpi>(a, p + c0 + e, o, kEpi == kAdapter && kN == kAdd ? v[e] + add[e] : v[e]);
           }
         } else {  // every product has read the ring: it holds the sums now
 #pragma unroll
@@ -288,10 +318,21 @@ __global__ void __launch_bounds__(kThreads) thin_kernel(const __grid_constant__ 
       cluster_sync();
       if (warp >= 2 && o < a.O) {
         const uint32_t part = ring0 + 4u * static_cast<uint32_t>(32 * (warp & 3) + lane);
-        for (int r = rank; r < rows; r += split) {
-          float v = 0.0f;
-          for (int q = 0; q < split; ++q) v += load_peer(part + 4u * kM * r, static_cast<uint32_t>(q));
-          put<kEpi>(a, p + r, o, v);
+        if (kEpi == kAdapter) {
+#pragma unroll
+          for (int j = 0; j < kAdd; ++j) {
+            const int r = rank + j * split;
+            if (r >= rows) break;
+            float v = 0.0f;
+            for (int q = 0; q < split; ++q) v += load_peer(part + 4u * kM * r, static_cast<uint32_t>(q));
+            put<kEpi>(a, p + r, o, v + add[j]);
+          }
+        } else {
+          for (int r = rank; r < rows; r += split) {
+            float v = 0.0f;
+            for (int q = 0; q < split; ++q) v += load_peer(part + 4u * kM * r, static_cast<uint32_t>(q));
+            put<kEpi>(a, p + r, o, v);
+          }
         }
       }
       fence_proxy_async();  // the ring's next writer is TMA
