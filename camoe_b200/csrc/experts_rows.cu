@@ -8,12 +8,16 @@
 //
 // Up to kSmallSlots slots one launch does it all: each token's block counts its
 // own slots' rows by reading the whole index once (a warp per slot) and copies
-// its row.  Above that: counts per chunk of 1024 slots, one scan over (expert,
-// chunk), the rows of each chunk's slots, and the copy.
+// its row.  Above that the slots are counted per chunk, every chunk's block places
+// its own slots (adding up the counts of the chunks before it, and a warp's of the
+// warps before it), and the copy follows; the launches overlap (programmatic
+// dependent launches), so that the index and x are loaded by the time the counts
+// and the rows are known.
 //
-// The copies are bound by HBM: a thread holds 16 bytes of a row (or one element
-// where the width or an address is no multiple of 16 bytes), a token's row is
-// read once and written k times.
+// The copies are bound by HBM: a thread holds 16 bytes (or one element where the
+// width or an address is no multiple of 16 bytes) of a row of each of kTokens
+// tokens, so that enough loads are in flight; a token's row is read once and
+// written k times.
 #include "camoe_experts.h"
 #include "wkv7_common.cuh"
 
@@ -27,7 +31,6 @@ namespace rows {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSmallSlots = 2048;
-constexpr int kChunkSlots = 1024;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxSlots = 64;  // per token
 constexpr unsigned kFull = 0xffffffffu;
@@ -159,155 +162,220 @@ __global__ void __launch_bounds__(kThreads) small_kernel(const P* __restrict__ x
   }
 }
 
-// slots of each expert in each chunk: counts[e * chunks + c]
+constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kSortDeep = 4;
+
+// slots per block, a multiple of kSortThreads: at most 256 blocks
+inline int64_t chunk_of(int64_t S) {
+  const int64_t c = ((S + 255) / 256 + kSortThreads - 1) / kSortThreads * kSortThreads;
+  return c > 2 * kSortThreads ? c : 2 * kSortThreads;
+}
+inline int64_t chunks_of(int64_t S) { return (S + chunk_of(S) - 1) / chunk_of(S); }
+
+// slots of each expert in each chunk: counts[chunk][expert]
 template <typename I>
-__global__ void __launch_bounds__(kThreads) count_kernel(const I* __restrict__ index,
-                                                         int* __restrict__ counts, int64_t S, int E) {
+__global__ void __launch_bounds__(kSortThreads) count_kernel(const I* __restrict__ index,
+                                                             int* __restrict__ counts, int64_t S,
+                                                             int64_t chunk, int E) {
   __shared__ int count[kMaxExperts + 1];
-  for (int e = threadIdx.x; e <= E; e += kThreads) count[e] = 0;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  for (int e = threadIdx.x; e <= E; e += kSortThreads) count[e] = 0;
   __syncthreads();
-  const int64_t s0 = static_cast<int64_t>(blockIdx.x) * kChunkSlots;
-#pragma unroll
-  for (int i = 0; i < kChunkSlots / kThreads; ++i) {
-    const int64_t s = s0 + i * kThreads + threadIdx.x;
-    if (s < S) atomicAdd(&count[bin_of(index, s, E)], 1);
-  }
+  const int64_t s0 = blockIdx.x * chunk, s1 = s0 + chunk < S ? s0 + chunk : S;
+  for (int64_t s = s0 + threadIdx.x; s < s1; s += kSortThreads) atomicAdd(&count[bin_of(index, s, E)], 1);
   __syncthreads();
-  for (int e = threadIdx.x; e <= E; e += kThreads)
-    counts[static_cast<int64_t>(e) * gridDim.x + blockIdx.x] = count[e];
+  for (int e = threadIdx.x; e <= E; e += kSortThreads)
+    counts[static_cast<int64_t>(blockIdx.x) * (E + 1) + e] = count[e];
 }
 
-// counts -> first row of each (expert, chunk), in place; offsets
-template <bool kKeep>
-__global__ void __launch_bounds__(kThreads) scan_kernel(int* __restrict__ counts,
-                                                        int* __restrict__ offsets, int64_t chunks,
-                                                        int64_t S, int E) {
-  constexpr int kPer = 8;
-  if (kKeep && threadIdx.x == 0) offsets[E + 1] = static_cast<int>(S);
-  const int64_t total = (E + 1) * chunks;
-  int carry = 0;
-  for (int64_t i0 = 0; i0 < total; i0 += kThreads * kPer) {
-    const int64_t first = i0 + threadIdx.x * kPer;
-    int c[kPer], mine = 0, all;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      c[i] = first + i < total ? counts[first + i] : 0;
-      mine += c[i];
-    }
-    int at = carry + block_scan(mine, &all);
-    carry += all;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if (first + i < total) {
-        counts[first + i] = at;
-        if ((first + i) % chunks == 0) offsets[(first + i) / chunks] = at;
-      }
-      at += c[i];
-    }
-  }
-}
-
-// the row of each slot of a chunk; row[s] = position, or -1 - row of an unused slot
+// The rows of a chunk's slots.  Warp w owns the w-th contiguous share of the
+// chunk; `seen` counts a warp's slots of each expert, then holds the rows of the
+// chunk before them.
 template <typename I, bool kKeep>
-__global__ void __launch_bounds__(kThreads) place_kernel(const I* __restrict__ index,
-                                                         const int* __restrict__ first,
-                                                         int* __restrict__ position,
-                                                         int* __restrict__ source, int64_t S, int E) {
-  constexpr int kSteps = kChunkSlots / kThreads;
-  extern __shared__ int seen[];  // [kWarps][E + 1]: slots of each expert in a warp's share
+__global__ void __launch_bounds__(kSortThreads)
+    place_kernel(const I* __restrict__ index, const int* counts, int* __restrict__ offsets,
+                 int* __restrict__ position, int* __restrict__ source, int64_t S, int64_t chunk, int E) {
+  extern __shared__ int seen[];  // [kSortWarps][E + 1], then [E + 1] all slots, [E + 1] those of earlier chunks
+  __shared__ int part[kSortWarps];
+  int *all = seen + kSortWarps * (E + 1), *first = all + E + 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < kWarps * (E + 1); i += kThreads) seen[i] = 0;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  for (int i = threadIdx.x; i < (kSortWarps + 2) * (E + 1); i += kSortThreads) seen[i] = 0;
   __syncthreads();
   int* mine = seen + warp * (E + 1);
-  const int64_t s0 = static_cast<int64_t>(blockIdx.x) * kChunkSlots + warp * (kSteps * 32) + lane;
-  int bin[kSteps], rank[kSteps];
+  const int64_t share = chunk / kSortWarps, s0 = blockIdx.x * chunk + warp * share;
+  const int64_t s1 = s0 + share < S ? s0 + share : S;
+  for (int64_t t = s0; t < s1; t += 32 * kSortDeep) {  // kSortDeep steps' loads at once
+    int bin[kSortDeep];
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int64_t s = s0 + 32 * i;
-    bin[i] = s < S ? bin_of(index, s, E) : -1;
+    for (int u = 0; u < kSortDeep; ++u) {
+      const int64_t s = t + 32 * u + lane;
+      bin[u] = s < s1 ? bin_of(index, s, E) : E + 1;
+    }
+#pragma unroll
+    for (int u = 0; u < kSortDeep; ++u)
+      if (bin[u] <= E) atomicAdd(&mine[bin[u]], 1);
   }
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const unsigned same = __match_any_sync(kFull, bin[i]);
-    const int before = __popc(same & ((1u << lane) - 1u));
-    const int old = bin[i] >= 0 ? mine[bin[i]] : 0;
-    rank[i] = old + before;
-    __syncwarp();
-    if (before == 0 && bin[i] >= 0) mine[bin[i]] = old + __popc(same);
-    __syncwarp();
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the counts
+  const int chunks = gridDim.x;
+  for (int i = threadIdx.x; i < chunks * (E + 1); i += kSortThreads) {
+    const int n = counts[i], c = i / (E + 1), e = i - c * (E + 1);
+    if (n == 0) continue;
+    atomicAdd(&all[e], n);
+    if (c < static_cast<int>(blockIdx.x)) atomicAdd(&first[e], n);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e <= E; e += kThreads) {
-    int at = first[static_cast<int64_t>(e) * gridDim.x + blockIdx.x];
-    for (int w = 0; w < kWarps; ++w) {
+  // rows before expert e: a scan over the experts, `per` of them per thread
+  const int per = (E + kSortThreads) / kSortThreads, e0 = threadIdx.x * per;
+  int n = 0;
+  for (int e = e0; e < e0 + per && e <= E; ++e) n += all[e];
+  int x = n;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(kFull, x, d);
+    if (lane >= d) x += y;
+  }
+  if (lane == 31) part[warp] = x;
+  __syncthreads();
+  int at = x - n;
+  for (int w = 0; w < warp; ++w) at += part[w];
+  for (int e = e0; e < e0 + per && e <= E; ++e) {
+    if (blockIdx.x == 0) offsets[e] = at;
+    first[e] += at;
+    at += all[e];
+  }
+  if (kKeep && blockIdx.x == 0 && threadIdx.x == 0) offsets[E + 1] = static_cast<int>(S);
+  __syncthreads();
+  for (int e = threadIdx.x; e <= E; e += kSortThreads) {
+    int r = first[e];
+    for (int w = 0; w < kSortWarps; ++w) {
       const int c = seen[w * (E + 1) + e];
-      seen[w * (E + 1) + e] = at;
-      at += c;
+      seen[w * (E + 1) + e] = r;
+      r += c;
     }
   }
   __syncthreads();
+  for (int64_t t = s0; t < s1; t += 32 * kSortDeep) {
+    int bin[kSortDeep];
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int64_t s = s0 + 32 * i;
-    if (bin[i] < 0) continue;
-    const int r = mine[bin[i]] + rank[i];
-    const bool used = kKeep || bin[i] < E;
-    position[s] = used ? r : -1;
-    source[r] = used ? static_cast<int>(s) : -1;
-  }
-}
-
-// ---- copies: blockDim.x threads along a row, blockDim.y tokens
-
-template <typename P>
-__global__ void __launch_bounds__(kThreads) copy_kernel(const P* __restrict__ x,
-                                                        const int* __restrict__ position,
-                                                        P* __restrict__ xs, int64_t N, int k, int64_t V) {
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
-  if (n >= N) return;
-  for (int64_t v = threadIdx.x; v < V; v += blockDim.x) {
-    const P p = x[n * V + v];
-    for (int j = 0; j < k; ++j) {
-      const int r = position[n * k + j];
-      if (r >= 0) xs[r * V + v] = p;  // below N k: the sort's own
+    for (int u = 0; u < kSortDeep; ++u) {
+      const int64_t s = t + 32 * u + lane;
+      bin[u] = s < s1 ? bin_of(index, s, E) : E + 1;
+    }
+#pragma unroll
+    for (int u = 0; u < kSortDeep; ++u) {
+      const unsigned same = __match_any_sync(kFull, bin[u]);
+      const int ahead = __popc(same & ((1u << lane) - 1u));
+      const int r = bin[u] <= E ? mine[bin[u]] + ahead : 0;
+      __syncwarp();
+      if (bin[u] <= E && ahead == 0) mine[bin[u]] += __popc(same);
+      __syncwarp();
+      if (bin[u] > E) continue;
+      const bool used = kKeep || bin[u] < E;
+      const int64_t s = t + 32 * u + lane;
+      position[s] = used ? r : -1;
+      source[r] = used ? static_cast<int>(s) : -1;
     }
   }
 }
 
-// zeros in the rows behind offsets[E]
+// ---- copies: blockDim.x threads along a row, blockDim.y groups of kTokens tokens
+// kTokens apart; the first kTailBlocks blocks write zeros behind offsets[E].
+
+constexpr int kTokens = 2, kTailBlocks = 148;
+
 template <typename P>
-__global__ void __launch_bounds__(kThreads) tail_kernel(const int* __restrict__ offsets, int E,
-                                                        P* __restrict__ xs, int64_t R, int64_t V) {
-  const int64_t end = R * V;
+__device__ __forceinline__ void zero_rows(const int* offsets, int E, P* rows, int64_t R, int64_t V) {
+  const int64_t threads = static_cast<int64_t>(blockDim.x) * blockDim.y;
   const int64_t used = offsets[E] > 0 ? offsets[E] : 0;
-  for (int64_t i = used * V + static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < end;
-       i += static_cast<int64_t>(gridDim.x) * kThreads)
-    xs[i] = zero_piece<P>();
+  for (int64_t i = used * V + blockIdx.x * threads + threadIdx.y * blockDim.x + threadIdx.x; i < R * V;
+       i += kTailBlocks * threads)
+    rows[i] = zero_piece<P>();
 }
 
-template <typename T, typename P, bool kWeighted>
+template <typename P>
+__global__ void __launch_bounds__(kThreads) copy_kernel(const P* __restrict__ x, const int* position,
+                                                        const int* offsets, P* __restrict__ xs, int64_t N, int k,
+                                                        int E, int64_t V, bool tail) {
+  if (tail && blockIdx.x < kTailBlocks) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    zero_rows(offsets, E, xs, N * k, V);
+    return;
+  }
+  const int64_t n0 = (static_cast<int64_t>(blockIdx.x) - (tail ? kTailBlocks : 0)) * (blockDim.y * kTokens) + threadIdx.y;
+  for (int64_t v = threadIdx.x; v < V; v += blockDim.x) {
+    P p[kTokens];
+#pragma unroll
+    for (int u = 0; u < kTokens; ++u) {
+      const int64_t n = n0 + u * blockDim.y;
+      p[u] = n < N ? x[n * V + v] : zero_piece<P>();
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the sort, which the loads of x do not need
+    for (int j0 = 0; j0 < k; j0 += 4) {  // the rows of four slots, then their stores
+      int r[kTokens][4];
+#pragma unroll
+      for (int u = 0; u < kTokens; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t n = n0 + u * blockDim.y;
+          r[u][j] = n < N && j0 + j < k ? position[n * k + j0 + j] : -1;
+        }
+#pragma unroll
+      for (int u = 0; u < kTokens; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (r[u][j] >= 0) xs[r[u][j] * V + v] = p[u];  // below N k: the sort's own
+    }
+  }
+}
+
+// kPer tokens per thread
+template <typename T, typename P, bool kWeighted, int kPer>
 __global__ void __launch_bounds__(kThreads) combine_kernel(const P* __restrict__ rows,
                                                            const float* __restrict__ weight,
                                                            const int* __restrict__ position,
                                                            P* __restrict__ out, int64_t N, int k,
                                                            int64_t V) {
   constexpr int n_el = Piece<T, P>::n;
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
-  if (n >= N) return;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (blockDim.y * kPer) + threadIdx.y;
   for (int64_t v = threadIdx.x; v < V; v += blockDim.x) {
-    float acc[n_el];
+    float acc[kPer][n_el];
 #pragma unroll
-    for (int i = 0; i < n_el; ++i) acc[i] = 0.0f;
-    for (int j = 0; j < k; ++j) {
-      const int64_t r = position[n * k + j];
-      if (r < 0 || r >= N * k) continue;
-      float f[n_el];
-      widen<T, P>(rows[r * V + v], f);
-      const float w = kWeighted ? weight[n * k + j] : 1.0f;
+    for (int u = 0; u < kPer; ++u)
 #pragma unroll
-      for (int i = 0; i < n_el; ++i) acc[i] = kWeighted ? fmaf(w, f[i], acc[i]) : acc[i] + f[i];
+      for (int i = 0; i < n_el; ++i) acc[u][i] = 0.0f;
+    for (int j0 = 0; j0 < k; j0 += 2) {  // the loads of two slots of all tokens, then their sums
+      int64_t r[kPer][2];
+      P p[kPer][2];
+#pragma unroll
+      for (int u = 0; u < kPer; ++u)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int64_t n = n0 + u * blockDim.y;
+          r[u][j] = n < N && j0 + j < k ? position[n * k + j0 + j] : -1;
+          if (r[u][j] >= N * k) r[u][j] = -1;
+        }
+#pragma unroll
+      for (int u = 0; u < kPer; ++u)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (r[u][j] >= 0) p[u][j] = rows[r[u][j] * V + v];
+#pragma unroll
+      for (int u = 0; u < kPer; ++u)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (r[u][j] < 0) continue;
+          float f[n_el];
+          widen<T, P>(p[u][j], f);
+          const float w = kWeighted ? weight[(n0 + u * blockDim.y) * k + j0 + j] : 1.0f;
+#pragma unroll
+          for (int i = 0; i < n_el; ++i) acc[u][i] = kWeighted ? fmaf(w, f[i], acc[u][i]) : acc[u][i] + f[i];
+        }
     }
-    out[n * V + v] = narrow<T, P>(acc);
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int64_t n = n0 + u * blockDim.y;
+      if (n < N) out[n * V + v] = narrow<T, P>(acc[u]);
+    }
   }
 }
 
@@ -315,11 +383,15 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const P* __restrict__
 template <typename T, typename P>
 __global__ void __launch_bounds__(kThreads) combine_bwd_kernel(
     const P* __restrict__ dout, const P* __restrict__ ys, const float* __restrict__ weight,
-    const int* __restrict__ position, P* __restrict__ dys, float* __restrict__ dweight, int64_t N,
-    int k, int64_t V) {
-  constexpr int n_el = Piece<T, P>::n, kGroup = 4;
+    const int* __restrict__ position, const int* __restrict__ offsets, P* __restrict__ dys,
+    float* __restrict__ dweight, int64_t N, int k, int E, int64_t V) {
+  constexpr int n_el = Piece<T, P>::n, kGroup = 2, kDeep = 4;
+  if (dys != nullptr && blockIdx.x < kTailBlocks) {
+    zero_rows(offsets, E, dys, N * k, V);
+    return;
+  }
   const int lane = threadIdx.x & 31;
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const int64_t n = (static_cast<int64_t>(blockIdx.x) - (dys != nullptr ? kTailBlocks : 0)) * kWarps + (threadIdx.x >> 5);
   if (n >= N) return;
   for (int j0 = 0; j0 < k; j0 += kGroup) {
     int64_t r[kGroup];
@@ -331,23 +403,37 @@ __global__ void __launch_bounds__(kThreads) combine_bwd_kernel(
       w[j] = r[j] >= 0 ? weight[n * k + j0 + j] : 0.0f;
       dot[j] = 0.0f;
     }
-    for (int64_t v = lane; v < V; v += 32) {
-      float d[n_el];
-      widen<T, P>(dout[n * V + v], d);
+    for (int64_t v0 = lane; v0 < V; v0 += 32 * kDeep) {
+      P d[kDeep], y[kDeep][kGroup];
 #pragma unroll
-      for (int j = 0; j < kGroup; ++j) {
-        if (r[j] < 0) continue;
-        if (dweight != nullptr) {
-          float f[n_el];
-          widen<T, P>(ys[r[j] * V + v], f);
+      for (int u = 0; u < kDeep; ++u) {
+        const int64_t v = v0 + 32 * u;
+        if (v >= V) continue;
+        d[u] = dout[n * V + v];
 #pragma unroll
-          for (int i = 0; i < n_el; ++i) dot[j] = fmaf(d[i], f[i], dot[j]);
-        }
-        if (dys != nullptr) {
+        for (int j = 0; j < kGroup; ++j)
+          if (r[j] >= 0 && dweight != nullptr) y[u][j] = ys[r[j] * V + v];
+      }
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u) {
+        const int64_t v = v0 + 32 * u;
+        if (v >= V) continue;
+        float df[n_el];
+        widen<T, P>(d[u], df);
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) {
+          if (r[j] < 0) continue;
           float g[n_el];
+          if (dweight != nullptr) {
+            widen<T, P>(y[u][j], g);
 #pragma unroll
-          for (int i = 0; i < n_el; ++i) g[i] = w[j] * d[i];
-          dys[r[j] * V + v] = narrow<T, P>(g);
+            for (int i = 0; i < n_el; ++i) dot[j] = fmaf(df[i], g[i], dot[j]);
+          }
+          if (dys != nullptr) {
+#pragma unroll
+            for (int i = 0; i < n_el; ++i) g[i] = w[j] * df[i];
+            dys[r[j] * V + v] = narrow<T, P>(g);
+          }
         }
       }
     }
@@ -368,9 +454,7 @@ inline dim3 row_block(int64_t V) {
   while (tx < kThreads && tx < V) tx *= 2;
   return dim3(tx, kThreads / tx);
 }
-inline int64_t blocks(int64_t N, const dim3& b) { return (N + b.y - 1) / b.y; }
-
-inline int64_t chunks_of(int64_t S) { return (S + kChunkSlots - 1) / kChunkSlots; }
+inline int64_t blocks(int64_t N, const dim3& b, int per) { return (N + b.y * per - 1) / (b.y * per); }
 
 // C elements of 2 or 4 bytes as 16-byte pieces: 0 where that cannot be
 template <typename... Ptr>
@@ -389,26 +473,42 @@ int check(int64_t N, int64_t k, int64_t E, int64_t C, int dtype) {
 }
 
 template <typename I, typename P, bool kKeep>
-int sort(const P* x, const I* index, P* xs, int* offsets, int* position, int* source, int* work,
-         int64_t N, int k, int E, int64_t V, cudaStream_t st) {
+int sort(const P* x, const I* index, P* xs, int* offsets, int* position, int* source, int* work, int64_t N, int k, int E, int64_t V, cudaStream_t st) {
   const int64_t S = N * k;
   if (S <= kSmallSlots) {
     small_kernel<I, P, kKeep><<<static_cast<unsigned>(N + 1), kThreads, 0, st>>>(
         x, index, xs, offsets, position, source, static_cast<int>(N), k, E, V);
     return camoe::tm::status(cudaGetLastError());
   }
-  const int64_t chunks = chunks_of(S);
-  const unsigned g = static_cast<unsigned>(chunks);
-  count_kernel<I><<<g, kThreads, 0, st>>>(index, work, S, E);
-  scan_kernel<kKeep><<<1, kThreads, 0, st>>>(work, offsets, chunks, S, E);
-  place_kernel<I, kKeep><<<g, kThreads, kWarps * (E + 1) * sizeof(int), st>>>(index, work, position,
-                                                                             source, S, E);
-  if (xs != nullptr && V > 0) {
-    const dim3 b = row_block(V);
-    copy_kernel<P><<<static_cast<unsigned>(blocks(N, b)), b, 0, st>>>(x, position, xs, N, k, V);
-    if (!kKeep) tail_kernel<P><<<148, kThreads, 0, st>>>(offsets, E, xs, S, V);
-  }
-  return camoe::tm::status(cudaGetLastError());
+  const int64_t chunk = chunk_of(S);
+  const unsigned g = static_cast<unsigned>(chunks_of(S));
+  count_kernel<I><<<g, kSortThreads, 0, st>>>(index, work, S, chunk, E);
+  if (const int e = camoe::tm::status(cudaGetLastError())) return e;
+  const int smem = (kSortWarps + 2) * (E + 1) * static_cast<int>(sizeof(int));
+  const auto place = place_kernel<I, kKeep>;
+  if (smem > 48 * 1024)
+    if (const int e = camoe::tm::status(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))
+      return e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(g);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (const int e = camoe::tm::status(cudaLaunchKernelEx(&cfg, place, index, static_cast<const int*>(work), offsets,
+                                                         position, source, S, chunk, E)))
+    return e;
+  if (xs == nullptr || V == 0) return 0;
+  const dim3 b = row_block(V);
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks(N, b, kTokens) + (kKeep ? 0 : kTailBlocks)));
+  cfg.blockDim = b;
+  cfg.dynamicSmemBytes = 0;
+  return camoe::tm::status(cudaLaunchKernelEx(&cfg, copy_kernel<P>, x, static_cast<const int*>(position),
+                                              static_cast<const int*>(offsets), xs, N, k, E, V, !kKeep));
 }
 
 template <typename P>
@@ -440,13 +540,21 @@ template <typename T, typename P>
 int combine(const void* in, const float* weight, const int* position, void* out, int64_t N, int k,
             int64_t V, cudaStream_t st) {
   const dim3 b = row_block(V);
-  const unsigned g = static_cast<unsigned>(blocks(N, b));
-  if (weight != nullptr)
-    combine_kernel<T, P, true><<<g, b, 0, st>>>(static_cast<const P*>(in), weight, position,
-                                                static_cast<P*>(out), N, k, V);
-  else
-    combine_kernel<T, P, false><<<g, b, 0, st>>>(static_cast<const P*>(in), weight, position,
-                                                 static_cast<P*>(out), N, k, V);
+  const P* p = static_cast<const P*>(in);
+  P* o = static_cast<P*>(out);
+  // few tokens: one per thread, so that all SMs have some
+  const bool many = N >= 4096;
+  const unsigned g = static_cast<unsigned>(blocks(N, b, many ? 2 : 1));
+  if (weight != nullptr) {
+    if (many)
+      combine_kernel<T, P, true, 2><<<g, b, 0, st>>>(p, weight, position, o, N, k, V);
+    else
+      combine_kernel<T, P, true, 1><<<g, b, 0, st>>>(p, weight, position, o, N, k, V);
+  } else if (many) {
+    combine_kernel<T, P, false, 2><<<g, b, 0, st>>>(p, weight, position, o, N, k, V);
+  } else {
+    combine_kernel<T, P, false, 1><<<g, b, 0, st>>>(p, weight, position, o, N, k, V);
+  }
   return camoe::tm::status(cudaGetLastError());
 }
 
@@ -454,11 +562,10 @@ template <typename T, typename P>
 int combine_bwd(const void* dout, const void* ys, const float* weight, const int* offsets,
                 const int* position, void* dys, float* dweight, int64_t N, int k, int E, int64_t V,
                 cudaStream_t st) {
-  combine_bwd_kernel<T, P><<<static_cast<unsigned>((N + kWarps - 1) / kWarps), kThreads, 0, st>>>(
-      static_cast<const P*>(dout), static_cast<const P*>(ys), weight, position, static_cast<P*>(dys),
-      dweight, N, k, V);
-  if (dys != nullptr && V > 0)
-    tail_kernel<P><<<148, kThreads, 0, st>>>(offsets, E, static_cast<P*>(dys), N * k, V);
+  const int64_t g = (N + kWarps - 1) / kWarps + (dys != nullptr ? kTailBlocks : 0);
+  combine_bwd_kernel<T, P><<<static_cast<unsigned>(g), kThreads, 0, st>>>(
+      static_cast<const P*>(dout), static_cast<const P*>(ys), weight, position, offsets, static_cast<P*>(dys),
+      dweight, N, k, E, V);
   return camoe::tm::status(cudaGetLastError());
 }
 
@@ -483,7 +590,7 @@ int camoe_ex_dispatch(const void* x, int dtype, const void* index, int index_byt
   if (N == 0)
     return camoe::tm::status(cudaMemsetAsync(offsets, 0, static_cast<size_t>(E + 1) * sizeof(int), s));
   if (index == nullptr || position == nullptr || source == nullptr || (xs != nullptr && x == nullptr)) return 1;
-  const size_t need = camoe_ex_dispatch_work_bytes(N, k, E);
+  const size_t need = sort_bytes(N, k, E);
   if (need > 0 && work == nullptr) return 1;
   if (work_bytes < need) return 5;
   int* w = static_cast<int*>(work);

@@ -77,11 +77,11 @@ def _dispatch(x, index, E):
     N, C = x.shape
     k = index.shape[1]
     dev = x.device
-    lib = _lib.lib()
     xs = torch.empty(N * k, C, dtype=x.dtype, device=dev)
     offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
     position = torch.empty(N, k, dtype=torch.int32, device=dev)
     source = torch.empty(N * k, dtype=torch.int32, device=dev)
+    lib = _lib.lib()
     need = lib.camoe_ex_dispatch_work_bytes(N, k, E)
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None  # none for few tokens
     check(lib.camoe_ex_dispatch(x.data_ptr(), dtype_code(x.dtype), index.data_ptr(), index.element_size(),

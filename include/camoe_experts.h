@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-/* Bytes of workspace of camoe_ex_dispatch (0 where it needs none). */
+/* Bytes of workspace of camoe_ex_dispatch (0 for up to 2048 slots: work may be NULL). */
 size_t camoe_ex_dispatch_work_bytes(int64_t N, int64_t k, int64_t E);
 
 /* Sort the slots and copy the tokens: index [N, k] holds the chosen experts
