@@ -81,6 +81,8 @@ struct Shape {
   static constexpr int kFit = (kRingBytes - (kBufs - 1) * kEpiWarps * static_cast<int>(kOutBytes + kLowBytes)) / (kABytes + kBBytes);
   static constexpr int kStages = kFit < 10 ? kFit : 10;
   static constexpr uint32_t kStaging = kEpiWarps * kBufs * (kOutBytes + kLowBytes);
+  // columns of B in a TMA box: half of a CTA's share, or 64 where they are contiguous
+  __host__ __device__ static constexpr int box(bool mn) { return mn ? 64 : (kBN == 256 ? kBN / kCG / 2 : kBN / kCG); }
   static constexpr uint32_t kCols = 2 * kBN;              // two accumulators
 };
 
@@ -208,6 +210,12 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sm_addr(bar))
                  : "memory");
 }
+// true in one lane of the (converged) warp, the same one each time
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 template <int kCG>
@@ -257,7 +265,7 @@ __host__ __device__ constexpr uint32_t instr(int M, int N) {
 // ---- tiles
 
 struct Tile {
-  int group, n0;
+  int group, n0, width;  // width: columns, kBN or half of it
   int64_t row0, row1;  // the group's rows from the tile's first (weight gradients: all of the group's)
   int m0;              // weight gradients: first output row
   int nk1, nk;         // pieces of the first pair, of both
@@ -267,21 +275,30 @@ template <int kCG, int kBN, bool kWGrad>
 struct Tiles {
   const Args& a;
   const Control& c;
-  int nt, mt, total;
+  int nt, mt;
+  int whole, jobs;  // tiles done whole, and these with the halves of the others
   __device__ Tiles(const Args& args, const Control& ctl) : a(args), c(ctl) {
     nt = (a.N + kBN - 1) / kBN;
     mt = kWGrad ? (a.M + (128 * kCG) - 1) / (128 * kCG) : 0;
-    total = kWGrad ? a.groups * mt * nt : c.tiles[a.groups] * nt;
+    const int total = kWGrad ? a.groups * mt * nt : c.tiles[a.groups] * nt;
+    // Tiles left for a last round that would leave half of the workers or more
+    // without one are done as halves of kBN / 2 columns, which take half the time.
+    const int workers = gridDim.x / kCG, left = total % workers;
+    const bool halves = kBN == 256 && 2 * left <= workers;
+    whole = halves ? total - left : total;
+    jobs = halves ? whole + 2 * left : total;
   }
   // rows are clamped to R: whatever the offsets hold, nothing outside the arrays is touched
   __device__ int64_t first(int g) const {
     const int64_t o = a.offsets[g];
     return o < 0 ? 0 : (o < a.R ? o : a.R);
   }
-  __device__ Tile get(int t) const {
+  __device__ Tile get(int job) const {
     Tile x;
+    const int t = job < whole ? job : whole + (job - whole) / 2;
     const int rt = t / nt;
-    x.n0 = (t - rt * nt) * kBN;
+    x.width = job < whole ? kBN : kBN / 2;
+    x.n0 = (t - rt * nt) * kBN + (job < whole ? 0 : (job - whole) % 2 * (kBN / 2));
     if (kWGrad) {
       x.group = rt / mt;
       x.m0 = (rt - x.group * mt) * (128 * kCG);
@@ -341,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const __grid_constant__ CUtensorMap ma2, const __grid_constant__ CUtensorMap mb2,
                 const Args a) {
   using Sh = Shape<kCG, kBN, kEpi>;
-  constexpr int S = Sh::kStages, kBCols = kBN / kCG;
+  constexpr int S = Sh::kStages, kBBox = Sh::box(kBMN);
   constexpr uint32_t kStage = Sh::kABytes + Sh::kBBytes;
   extern __shared__ __align__(128) unsigned char raw[];
   unsigned char* ring = raw + ((1024u - (sm_addr(raw) & 1023u)) & 1023u);
@@ -398,32 +415,39 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = c.tmem, ring0 = sm_addr(ring);
   const Tiles<kCG, kBN, kWGrad> tiles(a, c);
 
+  // Producer and product issue run as whole warps of which an elected lane acts: with
+  // the operands uniform over the warp the issue is short (a branch on the lane
+  // number made a 64-deep piece of 256 x 128 outputs take 0.31 us, whatever its
+  // size; elected, 0.20 us).
   if (warp == 0) {
-    if (lane == 0) {
-      int i = 0;  // pieces loaded so far
-      bool ok = true;
-      for (int t = worker; ok && t < tiles.total; t += workers) {
-        const Tile x = tiles.get(t);
-        const int row = static_cast<int>(x.row0) + static_cast<int>(rank) * 128;
-        const int m = x.m0 + static_cast<int>(rank) * 128, n = x.n0 + static_cast<int>(rank) * kBCols;
-        const bool cut = kWGrad && ((x.row1 - x.row0) % kBK) != 0;
-        for (int j = 0; j < x.nk; ++j, ++i) {
-          const int s = i % S;
-          if (i >= S && !(ok = mbar_wait(&c.empty[s], static_cast<uint32_t>((i / S - 1) & 1)))) break;
+    int loaded = 0, s = 0;  // pieces loaded so far; their stage
+    uint32_t round = 0;     // of the ring
+    bool ok = true;
+    for (int t = worker; ok && t < tiles.jobs; t += workers) {
+      const Tile x = tiles.get(t);
+      const int row = static_cast<int>(x.row0) + static_cast<int>(rank) * 128;
+      const int m = x.m0 + static_cast<int>(rank) * 128, n = x.n0 + static_cast<int>(rank) * (x.width / kCG);
+      const bool two = x.width / kCG > kBBox;  // boxes of B beyond the first
+      const int boxes = x.width / kCG / kBBox;
+      const uint32_t bytes = Sh::kABytes + static_cast<uint32_t>(x.width / kCG) * 128u;
+      const bool cut = kWGrad && ((x.row1 - x.row0) % kBK) != 0;
+      for (int j = 0; j < x.nk; ++j) {
+        if (round > 0 && !(ok = warp_wait(&c.empty[s], (round - 1) & 1u))) break;
+        if (elect_one()) {
           const bool last = cut && j == x.nk - 1;
           // a piece to be cleared lands on this CTA's own barrier
           const uint32_t bar = last ? sm_addr(&c.tail[s]) : bar_at<kCG>(&c.full[s], 0);
           if (last)
-            mbar_arrive_expect_tx(&c.tail[s], kStage);
+            mbar_arrive_expect_tx(&c.tail[s], bytes);
           else if (rank == 0)  // for both CTAs: the pair's loads complete on the leader's barrier
-            mbar_arrive_expect_tx(&c.full[s], kCG * kStage);
+            mbar_arrive_expect_tx(&c.full[s], kCG * bytes);
           const uint32_t sa = ring0 + s * kStage, sb = sa + Sh::kABytes;
           if (kWGrad) {
             const int r = static_cast<int>(x.row0) + j * kBK;
             load_box<kCG>(sa, &ma, m, r, 0, bar);
             load_box<kCG>(sa + kBox, &ma, m + 64, r, 0, bar);
-#pragma unroll
-            for (int q = 0; q < kBCols / 64; ++q) load_box<kCG>(sb + q * kBox, &mb, n + 64 * q, r, 0, bar);
+            load_box<kCG>(sb, &mb, n, r, 0, bar);
+            for (int q = 1; q < boxes; ++q) load_box<kCG>(sb + q * kBox, &mb, n + 64 * q, r, 0, bar);
           } else {
             const bool one = j < x.nk1;
             const int k = (one ? j : j - x.nk1) * kBK;
@@ -432,40 +456,46 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int z = one && a.b_shared ? 0 : x.group;
             load_box<kCG>(sa, pa, k, row, 0, bar);
             if (kBMN) {
-#pragma unroll
-              for (int q = 0; q < kBCols / 64; ++q) load_box<kCG>(sb + q * kBox, pb, n + 64 * q, k, z, bar);
+              load_box<kCG>(sb, pb, n, k, z, bar);
+              for (int q = 1; q < boxes; ++q) load_box<kCG>(sb + q * kBox, pb, n + 64 * q, k, z, bar);
             } else {
               load_box<kCG>(sb, pb, k, n, z, bar);
+              if (two) load_box<kCG>(sb + kBBox * 128, pb, k, n + kBBox, z, bar);
             }
           }
         }
+        __syncwarp();
+        ++loaded;
+        if (++s == S) s = 0, ++round;
       }
-      // after a wait that ran out: this CTA's shared memory outlives the copies into it
-      if (!ok && rank == 0)
-        for (int q = i > S ? i - S : 0; q < i; ++q) mbar_wait(&c.full[q % S], static_cast<uint32_t>((q / S) & 1));
     }
+    // after a wait that ran out: this CTA's shared memory outlives the copies into it
+    if (!ok && rank == 0)
+      for (int q = loaded > S ? loaded - S : 0; q < loaded; ++q)
+        mbar_wait(&c.full[q % S], static_cast<uint32_t>((q / S) & 1));
   } else if (warp == 1) {
-    constexpr uint32_t idesc = instr<kAMN, kBMN>(Sh::kBM, kBN);
-    int i = 0, done = 0;
+    int done = 0, s = 0;
+    uint32_t round = 0;
     uint32_t tail_phase = 0;  // a bit per stage
     bool ok = true;
-    for (int t = worker; ok && t < tiles.total; t += workers) {
+    for (int t = worker; ok && t < tiles.jobs; t += workers) {
       const Tile x = tiles.get(t);
       const int tail = kWGrad ? static_cast<int>((x.row1 - x.row0) % kBK) : 0;
       if (x.nk == 0) continue;
+      const uint32_t idesc = x.width == kBN ? instr<kAMN, kBMN>(Sh::kBM, kBN) : instr<kAMN, kBMN>(Sh::kBM, kBN / 2);
+      const int boxes = static_cast<int>((Sh::kABytes + static_cast<uint32_t>(x.width / kCG) * 128u) / kBox);
       const int b = done & 1;
       if (rank == 0) {
         if (done >= 2 && !(ok = warp_wait(&c.acc_empty[b], static_cast<uint32_t>((done / 2 - 1) & 1)))) break;
         fence_after();
       }
-      for (int j = 0; j < x.nk; ++j, ++i) {
-        const int s = i % S;
+      for (int j = 0; j < x.nk; ++j) {
         const uint32_t sa = ring0 + s * kStage;
         if (kWGrad && tail != 0 && j == x.nk - 1) {
           if (!(ok = warp_wait(&c.tail[s], (tail_phase >> s) & 1u))) break;
           tail_phase ^= 1u << s;
 #pragma unroll 1
-          for (int q = 0; q < static_cast<int>(kStage / kBox); ++q)
+          for (int q = 0; q < boxes; ++q)
             for (uint32_t o = tail * 128 + lane * 16; o < kBox; o += 512)
               *reinterpret_cast<uint4*>(ring + s * kStage + q * kBox + o) = make_uint4(0u, 0u, 0u, 0u);
           fence_proxy_async();
@@ -480,24 +510,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
           }
         }
-        if (rank != 0) continue;
-        if (!(ok = warp_wait(&c.full[s], static_cast<uint32_t>((i / S) & 1)))) break;
-        fence_after();
-        if (lane == 0) {
+        if (rank == 0) {
+          if (!(ok = warp_wait(&c.full[s], round & 1u))) break;
+          fence_after();
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kBK / 16; ++k)
-            mma<kCG>(tmem + static_cast<uint32_t>(b * kBN), desc<kAMN>(sa + kStep<kAMN> * k),
-                     desc<kBMN>(sa + Sh::kABytes + kStep<kBMN> * k), idesc, j > 0 || k > 0);
-          commit<kCG>(&c.empty[s]);
+            for (int k = 0; k < kBK / 16; ++k)
+              mma<kCG>(tmem + static_cast<uint32_t>(b * kBN), desc<kAMN>(sa + kStep<kAMN> * k),
+                       desc<kBMN>(sa + Sh::kABytes + kStep<kBMN> * k), idesc, j > 0 || k > 0);
+            commit<kCG>(&c.empty[s]);
+            if (j == x.nk - 1) commit<kCG>(&c.acc_full[b]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (++s == S) s = 0, ++round;
       }
-      if (rank == 0 && ok && lane == 0) commit<kCG>(&c.acc_full[b]);
-      __syncwarp();
       ++done;
     }
-    if (!ok && rank == 0 && lane == 0) {  // the products in flight end before tensor memory is freed
-      commit<kCG>(&c.drained);
+    if (!ok && rank == 0) {  // the products in flight end before tensor memory is freed
+      if (elect_one()) commit<kCG>(&c.drained);
       mbar_wait(&c.drained, 0);
     }
     __syncwarp();
@@ -518,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     int done = 0;
     bool ok = true;
-    for (int t = worker; ok && t < tiles.total; t += workers) {
+    for (int t = worker; ok && t < tiles.jobs; t += workers) {
       const Tile x = tiles.get(t);
       const int b = done & 1;
       const bool have = x.nk > 0;
@@ -530,8 +561,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float scale = kEpi == kScale && a.scale != nullptr ? a.scale[x.group] : 1.0f;
       int to = 0;  // where this lane's row goes
       if (!kWGrad && a.scatter != nullptr && lane < rows) to = a.scatter[row0 + lane];
-      const int cols = a.N - x.n0 < (half + 1) * (kBN / 2) ? a.N - x.n0 : (half + 1) * (kBN / 2);
-      const int begin = half * (kBN / 2);
+      const int begin = half * (x.width / 2), end = begin + x.width / 2;
+      const int cols = a.N - x.n0 < end ? a.N - x.n0 : end;
       if (kEpi == kDRelu2 && rows > 0 && begin < cols) fetch(steps, x.n0 + begin, row0);
       if (have && !(ok = warp_wait(&c.acc_full[b], static_cast<uint32_t>((done / 2) & 1)))) break;
       fence_after();

@@ -47,7 +47,7 @@ int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2,
   using Sh = Shape<kCG, kBN, kEpi>;
   if (!tma::bind_context()) return camoe::tm::status(cudaErrorNoDevice);
   CUtensorMap m[4];
-  const int ra = kAMN ? 64 : 128, rb = kBMN ? 64 : kBN / kCG;
+  const int ra = kAMN ? 64 : 128, rb = Sh::box(kBMN);
   bool ok = tma::encode_3d_sw128(&m[0], A.base, A.inner, A.rows, A.depth, ra) &&
             tma::encode_3d_sw128(&m[1], B.base, B.inner, B.rows, B.depth, rb);
   if (kEpi == kDRelu2)  // A2: h, B2: low, in the epilogue's boxes of 32 rows
@@ -66,7 +66,7 @@ int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2,
   if (nt * rt > 0x7fffffffLL) return 3;  // CAMOE_ERR_SHAPE
   int64_t pairs = sm_count() / kCG;
   if (pairs < 1) return camoe::tm::status(cudaErrorNoDevice);
-  if (nt * rt < pairs) pairs = nt * rt > 0 ? nt * rt : 1;
+  if (2 * nt * rt < pairs) pairs = nt * rt > 0 ? 2 * nt * rt : 1;  // a tile may be done as two halves
   const auto kernel = gemm_kernel<kCG, kBN, kAMN, kBMN, kWGrad, kEpi>;
   static std::atomic<uint64_t> opted{0};
   constexpr int smem = smem_bytes<kCG, kBN, kEpi>();
