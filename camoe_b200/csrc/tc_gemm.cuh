@@ -370,6 +370,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int worker = blockIdx.x / kCG, workers = gridDim.x / kCG;
 
   if (tid == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&ma)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mb)) : "memory");
     for (int s = 0; s < S; ++s) {
       mbar_init(&c.full[s], 1);
       mbar_init(&c.empty[s], 1);
@@ -386,6 +388,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_fence_init();
   }
   if (warp == 1) tmem_alloc<kCG>(&c.tmem, Sh::kCols);
+  // Up to here the kernel may run beside the one before it in the stream
+  // (programmatic dependent launch); what follows reads what that one wrote.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!kWGrad && warp == 2) {  // row tiles of each group
     int carry = 0;
     for (int g0 = 0; g0 < a.groups; g0 += 32) {
