@@ -46,17 +46,29 @@ __global__ void __launch_bounds__(kThreads) low_kernel(const bf16* __restrict__ 
   const int a = adapter[n];
   if (a < 0 || a >= L || d >= D) return;
   const uint4* xp = reinterpret_cast<const uint4*>(x + static_cast<int64_t>(n) * C);
-  const bf16* dp = down + (static_cast<int64_t>(a) * D + d) * C;
+  const uint4* dp = reinterpret_cast<const uint4*>(down + (static_cast<int64_t>(a) * D + d) * C);
+  constexpr int kDeep = 4;  // loads in flight
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   float s = 0.0f;
-  for (int v = lane; v < C / 8; v += 32) {
-    const uint4 p = xp[v], q = *reinterpret_cast<const uint4*>(dp + 8 * v);
-    const __nv_bfloat162* ph = reinterpret_cast<const __nv_bfloat162*>(&p);
-    const __nv_bfloat162* qh = reinterpret_cast<const __nv_bfloat162*>(&q);
+  for (int v0 = lane; v0 < C / 8; v0 += 32 * kDeep) {
+    uint4 p[kDeep], q[kDeep];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = __bfloat1622float2(ph[e]), g = __bfloat1622float2(qh[e]);
-      s = fmaf(f.x, g.x, s);
-      s = fmaf(f.y, g.y, s);
+    for (int u = 0; u < kDeep; ++u) {
+      const bool in = v0 + 32 * u < C / 8;
+      p[u] = in ? xp[v0 + 32 * u] : zero;
+      q[u] = in ? dp[v0 + 32 * u] : zero;
+    }
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      if (v0 + 32 * u >= C / 8) continue;
+      const __nv_bfloat162* ph = reinterpret_cast<const __nv_bfloat162*>(&p[u]);
+      const __nv_bfloat162* qh = reinterpret_cast<const __nv_bfloat162*>(&q[u]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = __bfloat1622float2(ph[e]), g = __bfloat1622float2(qh[e]);
+        s = fmaf(f.x, g.x, s);
+        s = fmaf(f.y, g.y, s);
+      }
     }
   }
 #pragma unroll

@@ -32,11 +32,11 @@ namespace ffn {
 
 // Few rows per expert: the weights' bytes decide, and tiles of a few rows read them
 // at HBM rate; with more the products count, and 256-row tiles are faster.
-bool few_rows(int64_t R, int64_t E) { return R <= 64 * E; }
+bool few_rows(int64_t R, int64_t E) { return R <= 32 * E; }
 
-// Both products of 8 experts of 1024 x 4096 (134 MB): 28.6 us for 4 rows each (16 at a
-// time), 30.8 us for 16 and 36.6 us for 64 rows each (64 at a time), 31.5 us for
-// 2 to 44 and 53 us for 12 to 170 rows; the large tiles 53 to 56 us for all.
+// Both products of 8 experts of 1024 x 4096 (134 MB), us for 16, 32 and 64 rows each and
+// for as many rows unevenly spread: 32 (35), 35 (38) and 42 (66) here, 43, 44 and
+// 45 for all in 256-row tiles.
 template <int kEpi>
 int thin_product(const bf16* x, const bf16* w, const int* offsets, bf16* out, int8_t* low, int64_t R, int64_t E,
                  int64_t O, int64_t K, bool second, cudaStream_t st) {
@@ -50,8 +50,9 @@ int thin_product(const bf16* x, const bf16* w, const int* offsets, bf16* out, in
   a.out = out;
   a.low = low;
   const int64_t groups = E < R ? E : R;
-  // up to four rows per expert on average: 16 at a time; otherwise 64.  Two row
-  // tiles start side by side, for the experts with more rows than that.
+  // Up to four rows per expert on average: 16 at a time (24.5 us against 26.8 for 1 to
+  // 18 rows each); otherwise 64 (30.5 against 38.4 with 32, for 2 to 44 rows).  Two
+  // row tiles start side by side, for the experts with more rows than that.
   if (R <= 16) return thin::launch<16, kEpi>(x, w, a, groups, 1, st);
   if (R <= 4 * E) return thin::launch<16, kEpi>(x, w, a, groups, 2, st);
   return thin::launch<64, kEpi>(x, w, a, groups, R <= 64 ? 1 : 2, st);

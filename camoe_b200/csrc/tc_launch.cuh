@@ -114,13 +114,13 @@ int launch(const void* x, const void* w, Args a, int64_t groups, int64_t row_til
   a.split = split_of(tiles * groups * row_tiles, a.K, kN <= 64 ? 2 : 1, kEpi == kAdapter ? kN / kAdd : 1);
   const auto kernel = thin_kernel<kN, kEpi>;
   static std::atomic<uint64_t> opted{0};
-  constexpr int smem = smem_bytes<kN>();
-  if (const int st = camoe::tm::status(tc::allow_smem(kernel, smem, opted))) return st;
+  if (const int st = camoe::tm::status(tc::allow_smem(kernel, smem_bytes<kN>(kEpi == kAdapter ? 256 : 0), opted)))
+    return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * a.split), static_cast<unsigned>(groups),
                      static_cast<unsigned>(row_tiles));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = smem_bytes<kN>(kEpi == kAdapter ? a.D : 0);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;

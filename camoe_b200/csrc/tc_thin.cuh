@@ -58,9 +58,11 @@ struct Control {
   uint64_t full[kMaxStages], empty[kMaxStages], acc;
   uint32_t tmem;
 };
+// plus kAdapter's rows of low_rank
 template <int kN>
-__host__ __device__ constexpr int smem_bytes() {
-  return Shape<kN>::kStages * static_cast<int>(Shape<kN>::kStage) + static_cast<int>(sizeof(Control)) + 1024;
+__host__ __device__ constexpr int smem_bytes(int rank) {
+  return Shape<kN>::kStages * static_cast<int>(Shape<kN>::kStage) + static_cast<int>(sizeof(Control)) + 1024 +
+         16 * rank * static_cast<int>(sizeof(float));
 }
 
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -73,8 +75,7 @@ __device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
   asm volatile(
       "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.f32 %0, [a];\n}\n"
       : "=f"(v)
-      : "r"(addr), "r"(rank)
-      : "memory");
+      : "r"(addr), "r"(rank));
   return v;
 }
 
@@ -123,51 +124,68 @@ __device__ __forceinline__ void put(const Args& a, int64_t p, int o, float v) {
 }
 
 // kAdapter: what the adapters add to output o of up to kAdd rows p, p + step, ...
-// below end; four rows at a time, so that their loads overlap.
+// below end.  Four rows at a time and 16 columns of up each, so that their loads
+// overlap; `low` is those rows' low_rank in shared memory ([kAdd][D]).
 constexpr int kAdd = 16;
-__device__ __forceinline__ void adapter_add(const Args& a, int64_t p, int step, int64_t end, int o, float (&add)[kAdd]) {
+__device__ __forceinline__ void adapter_add(const Args& a, int64_t p, int step, int64_t end, int o, const float* low,
+                                            float (&add)[kAdd]) {
 #pragma unroll
   for (int r = 0; r < kAdd; r += 4) {
     const uint4* u[4];
-    const float4* l[4];
-    bool has[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t q = p + static_cast<int64_t>(step) * (r + j);
       const int ad = q < end && o < a.O ? a.adapter[q] : -1;
-      has[j] = ad >= 0 && ad < a.L;
-      u[j] = reinterpret_cast<const uint4*>(a.up + (static_cast<int64_t>(has[j] ? ad : 0) * a.O + o) * a.D);
-      l[j] = reinterpret_cast<const float4*>(a.low_rank + q * a.D);
+      u[j] = ad >= 0 && ad < a.L ? reinterpret_cast<const uint4*>(a.up + (static_cast<int64_t>(ad) * a.O + o) * a.D)
+                                 : nullptr;
       add[r + j] = 0.0f;
     }
-    for (int d = 0; d < a.D / 8; ++d) {
-      uint4 w[4];
-      float4 l0[4], l1[4];
+    if (p + static_cast<int64_t>(step) * r >= end) continue;
+    for (int d = 0; d < a.D / 8; d += 2) {
+      uint4 w[4][2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (u[j] != nullptr && d + h < a.D / 8) w[j][h] = u[j][d + h];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (!has[j]) continue;
-        w[j] = u[j][d];
-        l0[j] = l[j][2 * d];
-        l1[j] = l[j][2 * d + 1];
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (!has[j]) continue;
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w[j]);
-        const float2 q0 = __bfloat1622float2(h[0]), q1 = __bfloat1622float2(h[1]), q2 = __bfloat1622float2(h[2]),
-                     q3 = __bfloat1622float2(h[3]);
+        if (u[j] == nullptr) continue;
         float s = add[r + j];
-        s = fmaf(q0.x, l0[j].x, s);
-        s = fmaf(q0.y, l0[j].y, s);
-        s = fmaf(q1.x, l0[j].z, s);
-        s = fmaf(q1.y, l0[j].w, s);
-        s = fmaf(q2.x, l1[j].x, s);
-        s = fmaf(q2.y, l1[j].y, s);
-        s = fmaf(q3.x, l1[j].z, s);
-        s = fmaf(q3.y, l1[j].w, s);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (d + h >= a.D / 8) continue;
+          const float* l = low + (r + j) * a.D + 8 * (d + h);
+          const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&w[j][h]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = __bfloat1622float2(b[e]);
+            s = fmaf(f.x, l[2 * e], s);
+            s = fmaf(f.y, l[2 * e + 1], s);
+          }
+        }
         add[r + j] = s;
       }
     }
+  }
+}
+
+// The sums over the cluster of rows r, r + split, ... (those below `rows`), rank by
+// rank; all loads of kPeerRows rows are in flight at once.
+constexpr int kPeerRows = 4;
+__device__ __forceinline__ void peer_sums(uint32_t part, int r, int split, int rows, float (&v)[kPeerRows]) {
+  float x[kPeerRows][8];
+#pragma unroll
+  for (int e = 0; e < kPeerRows; ++e)
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      x[e][q] = q < split && r + e * split < rows ? load_peer(part + 4u * kM * (r + e * split), static_cast<uint32_t>(q))
+                                                  : 0.0f;
+#pragma unroll
+  for (int e = 0; e < kPeerRows; ++e) {
+    v[e] = x[e][0];
+#pragma unroll
+    for (int q = 1; q < 8; ++q) v[e] += x[e][q];
   }
 }
 
@@ -284,7 +302,13 @@ __global__ void __launch_bounds__(kThreads) thin_kernel(const __grid_constant__ 
     if (warp >= 2) {
       if (kEpi == kAdapter) {  // while the weights arrive
         wait_previous();       // low_rank
-        adapter_add(a, p + rank, split, r1 < p + kN ? r1 : p + kN, o, add);
+        float* low = reinterpret_cast<float*>(ring + S * Sh::kStage + sizeof(Control));
+        const int64_t end = r1 < p + kN ? r1 : p + kN;
+        named_sync(1, 128);  // the last row tile's are no longer read
+        for (int q = 0; q < kAdd && p + rank + q * split < end; ++q)
+          for (int d = tid - 64; d < a.D; d += 128) low[q * a.D + d] = a.low_rank[(p + rank + q * split) * a.D + d];
+        named_sync(1, 128);
+        adapter_add(a, p + rank, split, end, o, low, add);
       }
       if (k1 > k0) ok = tc::warp_wait(&c.acc, static_cast<uint32_t>(it & 1)) && ok;
       tc::fence_after();
@@ -320,18 +344,21 @@ __global__ void __launch_bounds__(kThreads) thin_kernel(const __grid_constant__ 
         const uint32_t part = ring0 + 4u * static_cast<uint32_t>(32 * (warp & 3) + lane);
         if (kEpi == kAdapter) {
 #pragma unroll
-          for (int j = 0; j < kAdd; ++j) {
-            const int r = rank + j * split;
-            if (r >= rows) break;
-            float v = 0.0f;
-            for (int q = 0; q < split; ++q) v += load_peer(part + 4u * kM * r, static_cast<uint32_t>(q));
-            put<kEpi>(a, p + r, o, v + add[j]);
+          for (int j = 0; j < kAdd; j += kPeerRows) {
+            if (rank + j * split >= rows) break;
+            float v[kPeerRows];
+            peer_sums(part, rank + j * split, split, rows, v);
+#pragma unroll
+            for (int e = 0; e < kPeerRows; ++e)
+              if (rank + (j + e) * split < rows) put<kEpi>(a, p + rank + (j + e) * split, o, v[e] + add[j + e]);
           }
         } else {
-          for (int r = rank; r < rows; r += split) {
-            float v = 0.0f;
-            for (int q = 0; q < split; ++q) v += load_peer(part + 4u * kM * r, static_cast<uint32_t>(q));
-            put<kEpi>(a, p + r, o, v);
+          for (int r = rank; r < rows; r += kPeerRows * split) {
+            float v[kPeerRows];
+            peer_sums(part, r, split, rows, v);
+#pragma unroll
+            for (int e = 0; e < kPeerRows; ++e)
+              if (r + e * split < rows) put<kEpi>(a, p + r + e * split, o, v[e]);
           }
         }
       }
