@@ -128,6 +128,18 @@ def lib() -> ctypes.CDLL:
     return l
 
 
+def torch_ops():
+    """The torch calls of the expert layer and the adapters (csrc/torch_ops.cpp)."""
+    import importlib
+
+    import torch  # noqa: F401  (its libraries have to be loaded first)
+    try:
+        return importlib.import_module("._torch_ops", __package__)
+    except ImportError as e:
+        raise ImportError(f"{os.path.join(HERE, '_torch_ops.so')} does not load ({e}); build it with "
+                          "`python -m camoe_b200.build` (the operators have no other path)") from e
+
+
 def check(status: int) -> None:
     if status != OK:
         l = lib()

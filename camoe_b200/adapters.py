@@ -11,19 +11,12 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib
-from ._lib import check
-from .experts import _check, _stream
+from .experts import _check, _check_aligned, _torch_ops
 
 MAX_RANK, MAX_ADAPTERS = 256, 1024
 
 
-def adapter_linear(x: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: torch.Tensor,
-                   adapter: torch.Tensor, scale: torch.Tensor | None = None) -> torch.Tensor:
-    """x [N, C], weight [M, C] (``F.linear``'s layout), down [L, D, C], up
-    [L, M, D], all bf16, C, M and D multiples of 8 and D at most 256 (adapters
-    of a smaller rank are padded with zeros); adapter [N] int32, a row outside
-    [0, L) has none; scale [L] fp32, ones when not given.  Returns y [N, M]."""
+def _refuse(x, weight, down, up, adapter, scale):
     if x.dim() != 2 or weight.dim() != 2 or down.dim() != 3:
         raise ValueError(f"expected x [N, C], weight [M, C] and down [L, D, C], got {tuple(x.shape)}, "
                          f"{tuple(weight.shape)} and {tuple(down.shape)}")
@@ -38,16 +31,43 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up
     _check(adapter, "adapter", (N,), torch.int32, dev)
     if scale is not None:
         _check(scale, "scale", (L,), torch.float32, dev)
-    if C % 8 or M % 8 or D % 8 or min(C, M, D) == 0 or D > MAX_RANK or not 1 <= L <= MAX_ADAPTERS:
-        raise ValueError(f"C, M and D must be positive multiples of 8, D at most {MAX_RANK}, 1 to {MAX_ADAPTERS} "
-                         f"adapters, got C = {C}, M = {M}, D = {D}, L = {L}")
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, weight, down, up)):
         raise RuntimeError("adapter_linear has no backward: call it under torch.no_grad()")
-    lib = _lib.lib()
-    y = torch.empty(N, M, dtype=bf, device=dev)
-    need = lib.camoe_ad_work_bytes(N, C, M, D, L)
-    work = torch.empty(need, dtype=torch.uint8, device=dev)
-    check(lib.camoe_ad_linear(x.data_ptr(), weight.data_ptr(), down.data_ptr(), up.data_ptr(), adapter.data_ptr(),
-                              None if scale is None else scale.data_ptr(), y.data_ptr(), work.data_ptr(), need,
-                              N, C, M, D, L, _stream(x)))
+    _check_aligned(x, weight, down, up)
+    raise ValueError(f"C, M and D must be positive multiples of 8, D at most {MAX_RANK}, 1 to {MAX_ADAPTERS} "
+                     f"adapters, got C = {C}, M = {M}, D = {D}, L = {L}")
+
+
+def adapter_linear(x: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: torch.Tensor,
+                   adapter: torch.Tensor, scale: torch.Tensor | None = None) -> torch.Tensor:
+    """x [N, C], weight [M, C] (``F.linear``'s layout), down [L, D, C], up
+    [L, M, D], all bf16, C, M and D multiples of 8 and D at most 256 (adapters
+    of a smaller rank are padded with zeros); adapter [N] int32, a row outside
+    [0, L) has none; scale [L] fp32, ones when not given.  Returns y [N, M]."""
+    y = _torch_ops.adapter_linear(x, weight, down, up, adapter, scale)
+    if y is None:
+        _refuse(x, weight, down, up, adapter, scale)
     return y
+
+
+class AdapterSet:
+    """The low-rank adapters of L requests for some of a module's projections:
+    ``add("key", down [L, D, C], up [L, M, D], scale [L])`` per projection;
+    ``linear("key", x [..., C], weight [M, C], adapter [rows])`` runs that
+    projection, with its adapters where it has any."""
+
+    def __init__(self):
+        self._of = {}
+
+    def add(self, name: str, down: torch.Tensor, up: torch.Tensor, scale: torch.Tensor | None = None) -> "AdapterSet":
+        bf = torch.bfloat16
+        self._of[name] = (down.to(bf).contiguous(), up.to(bf).contiguous(),
+                          None if scale is None else scale.float().contiguous())
+        return self
+
+    def linear(self, name: str, x: torch.Tensor, weight: torch.Tensor, adapter: torch.Tensor) -> torch.Tensor:
+        if name not in self._of:
+            return torch.nn.functional.linear(x, weight)
+        down, up, scale = self._of[name]
+        y = adapter_linear(x.reshape(-1, x.shape[-1]).contiguous(), weight, down, up, adapter, scale)
+        return y.view(*x.shape[:-1], weight.shape[0])

@@ -328,7 +328,8 @@ class RWKV7TimeMix(nn.Module):
         return out, v_first, srep
 
     @torch.no_grad()
-    def forward_state(self, x: torch.Tensor, v_first: torch.Tensor | None = None, state=None):
+    def forward_state(self, x: torch.Tensor, v_first: torch.Tensor | None = None, state=None,
+                      adapters=None, adapter: torch.Tensor | None = None):
         """Inference over steps [t0, t0 + T) of each sequence, carrying the
         layer's state across calls, so that generating a token costs one step
         instead of a pass over the whole context (the reference re-runs the
@@ -337,7 +338,12 @@ class RWKV7TimeMix(nn.Module):
         step of x (the token shift's input), wkv [B, H, 64, 64] fp32 the WKV
         state.  Returns (out, v_first, state_representation, new_state); the
         outputs equal ``forward`` over the concatenated steps.  ``v_first``
-        (layers > 0) covers the same steps as x."""
+        (layers > 0) covers the same steps as x.
+
+        ``adapters`` (an ``adapters.AdapterSet`` with any of "receptance", "key",
+        "value" and "output") adds to each of those projections the low-rank
+        adapter of each sequence's request: ``adapter`` [B] int32, a sequence
+        outside [0, L) has none."""
         B, T, C = x.shape
         H = C // HEAD_SIZE
         dev = x.device
@@ -360,9 +366,16 @@ class RWKV7TimeMix(nn.Module):
         xr, xw, xk, xv, xa, xg = xs
         W = (lambda m: m.weight.to(_BF))
         P = (lambda t: t.to(_BF))
-        r = F.linear(xr, W(self.receptance)).contiguous()
-        k = F.linear(xk, W(self.key)).contiguous()
-        v = F.linear(xv, W(self.value)).contiguous()
+        if adapters is None:
+            lin = (lambda name, t: F.linear(t, W(getattr(self, name))))
+        else:
+            if adapter is None or tuple(adapter.shape) != (B,):
+                raise ValueError(f"adapters need the adapter of each sequence, [B] = [{B}] int32")
+            of_row = adapter.to(torch.int32).repeat_interleave(T) if T > 1 else adapter.to(torch.int32).contiguous()
+            lin = (lambda name, t: adapters.linear(name, t, W(getattr(self, name)).contiguous(), of_row))
+        r = lin("receptance", xr).contiguous()
+        k = lin("key", xk).contiguous()
+        v = lin("value", xv).contiguous()
         wl = (torch.tanh(xw @ P(self.w1)) @ P(self.w2)).contiguous()
         al = ((xa @ P(self.a1)) @ P(self.a2)).contiguous()
         g = (torch.sigmoid(xg @ P(self.g1)) @ P(self.g2)).contiguous()
@@ -391,7 +404,7 @@ class RWKV7TimeMix(nn.Module):
         z = torch.empty(B, T, C, dtype=_BF, device=dev)
         check(L.camoe_tm_post_fwd(_p(y), _p(r), _p(k_op), _p(v_op), _p(g), _p(r_k), _p(gx),
                                   _p(bx), _p(z), B, T, C, st))
-        out = F.linear(z, W(self.output))
+        out = lin("output", z)
         if self.layer_id == 0:
             v_first = v
         return out, v_first, srep, (x[:, -1].contiguous(), wkv_new)

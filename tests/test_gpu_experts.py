@@ -302,6 +302,38 @@ def test_results_repeat_bit_for_bit_and_on_another_stream():
         assert torch.equal(a[:528] if a.shape == xs.shape else a, b[:528] if b.shape == xs.shape else b)
 
 
+@pytest.mark.parametrize("tokens", [6, 1500])
+def test_the_operators_replay_from_a_cuda_graph(tokens):
+    """Their launches overlap (programmatic dependent launches): captured and replayed
+    on new inputs they give what the calls give."""
+    from camoe_b200 import adapters
+    C, F, E, k = 128, 256, 5, 2
+    x, index = rnd(tokens, C, seed=80), index_of(tokens, k, E, 81, 0.1)
+    w = rnd(tokens, k, seed=82, dtype=F32)
+    w_up, w_down = rnd(E, F, C, seed=83, scale=C ** -0.5), rnd(E, C, F, seed=84, scale=F ** -0.5)
+    proj, down, up = rnd(C, C, seed=85, scale=C ** -0.5), rnd(3, 8, C, seed=86, scale=C ** -0.5), rnd(3, C, 8, seed=87)
+    which = (torch.arange(tokens, device="cuda") % 4 - 1).to(torch.int32)
+
+    def run():
+        y = adapters.adapter_linear(x, proj, down, up, which)
+        xs, plan = experts.expert_dispatch(y, index, E)
+        return experts.expert_combine(experts.expert_ffn(xs, w_up, w_down, plan.offsets), w, plan)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    x.copy_(rnd(tokens, C, seed=88))
+    index.copy_(index_of(tokens, k, E, 89, 0.4))
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, run())
+
+
 def test_empty_inputs():
     offsets = torch.zeros(4, dtype=torch.int32, device="cuda")
     w_up, w_down = rnd(3, 16, 8, seed=60), rnd(3, 8, 16, seed=61)
