@@ -2,11 +2,11 @@
 // include/camoe_experts.h):
 //   y[n] = weight x[n] + scale[a] up[a] (down[a] x[n]),  a = adapter[n]
 //
-// Few rows (a token of each of many requests): two launches.  low[n] = scale[a]
-// down[a] x[n] in fp32, a warp per output; then the projection with the weights
-// streamed once (tc_thin.cuh; it starts while the first kernel runs), to whose
-// sums each output adds its row of up times low, in fp32, before the one
-// rounding.
+// Few rows (a token of each of many requests): two launches, or one for the fewest.
+// low[n] = scale[a] down[a] x[n] in fp32, a warp per output; then the projection
+// with the weights streamed once (tc_thin.cuh; it starts while the first kernel
+// runs), to whose sums each output adds its row of up times low, in fp32, before
+// the one rounding.
 //
 // Many rows (prompts): the rows are sorted by adapter, low = scale (xs down^T)
 // is one grouped product (rounded to bf16, the type of the next product's
@@ -80,6 +80,12 @@ __global__ void __launch_bounds__(kThreads) low_kernel(const bf16* __restrict__ 
 // row tiles of one adapter each would be mostly empty.
 bool few_rows(int64_t N, int64_t L) { return N <= 256 || N < 16 * L; }
 
+// A few rows whose low-rank parts are little work for each CTA of a cluster of four
+// (64 KB of down read at most): every tile of the projection works them out for
+// itself, in one launch.  B200, us here / with a launch of their own, N x C x D:
+// 1 x 1024 x 16 6.9 / 8.3, 8 x 1024 x 16 7.3 / 8.3, 1 x 2048 x 64 15.7 / 10.3.
+bool own_low(int64_t N, int64_t C, int64_t D) { return N <= 8 && (N + 3) / 4 * C * D <= 32 * 1024; }
+
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 
 struct Layout {  // of the workspace
@@ -149,10 +155,14 @@ int camoe_ad_linear(const void* x, const void* weight, const void* down, const v
   const bf16* xb = static_cast<const bf16*>(x);
   if (few_rows(N, L)) {
     float* low = static_cast<float*>(work);
-    for (int64_t n0 = 0; n0 < N; n0 += 32768) {  // grid.y holds 65535
-      const int64_t n = N - n0 < 32768 ? N - n0 : 32768;
-      low_kernel<<<dim3((d + 7) / 8, static_cast<unsigned>(n)), kThreads, 0, s>>>(
-          xb + n0 * C, static_cast<const bf16*>(down), adapter + n0, scale, low + n0 * D, c, d, l);
+    const bool own = own_low(N, C, D);
+    if (!own) {
+      for (int64_t n0 = 0; n0 < N; n0 += 32768) {  // grid.y holds 65535
+        const int64_t n = N - n0 < 32768 ? N - n0 : 32768;
+        low_kernel<<<dim3((d + 7) / 8, static_cast<unsigned>(n)), kThreads, 0, s>>>(
+            xb + n0 * C, static_cast<const bf16*>(down), adapter + n0, scale, low + n0 * D, c, d, l);
+      }
+      if (const int st = camoe::tm::status(cudaGetLastError())) return st;
     }
     thin::Args t{};
     t.groups = 1;
@@ -162,11 +172,13 @@ int camoe_ad_linear(const void* x, const void* weight, const void* down, const v
     t.out = static_cast<bf16*>(y);
     t.up = static_cast<const bf16*>(up);
     t.adapter = adapter;
-    t.low_rank = low;
+    t.low_rank = own ? nullptr : low;
+    t.x = xb;
+    t.down = static_cast<const bf16*>(down);
+    t.scale = scale;
     t.D = d;
     t.L = l;
-    if (const int st = camoe::tm::status(cudaGetLastError())) return st;
-    t.second = 1;
+    t.second = own ? 0 : 1;  // the first kernel has waited for what is before it
     // row tiles of 32 started apart: their adapters' work runs side by side, and
     // the weights of all but one come from L2
     return N <= 16 ? thin::launch<16, thin::kAdapter>(x, weight, t, 1, 1, s)

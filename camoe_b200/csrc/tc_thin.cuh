@@ -38,10 +38,13 @@ struct Args {
   int zero_tail;       // write zeros to the rows behind the last group
   bf16* out;
   int8_t* low;         // tc::kRelu2: as in tc_gemm.cuh, or null
-  // kAdapter: out += up[a] low_rank[p], a = adapter[p]
+  // kAdapter: out += up[a] low[p], a = adapter[p]; low is low_rank [R, D], or (null)
+  // scale[a] down[a] x[p], which the kernel works out
   const bf16* up;
   const int* adapter;
   const float* low_rank;
+  const bf16 *x, *down;
+  const float* scale;
   int D, L;
 };
 
@@ -124,47 +127,102 @@ __device__ __forceinline__ void put(const Args& a, int64_t p, int o, float v) {
 }
 
 // kAdapter: what the adapters add to output o of up to kAdd rows p, p + step, ...
-// below end.  Four rows at a time and 16 columns of up each, so that their loads
-// overlap; `low` is those rows' low_rank in shared memory ([kAdd][D]).
-constexpr int kAdd = 16;
-__device__ __forceinline__ void adapter_add(const Args& a, int64_t p, int step, int64_t end, int o, const float* low,
-                                            float (&add)[kAdd]) {
+// below end.  kAddRows rows at a time and 16 columns of up each, so that their
+// loads overlap; those of the first step are made by fetch(), before `low`, the
+// rows' low_rank in shared memory ([kAdd][D]), is there.
+constexpr int kAdd = 16, kAddRows = 8;
+struct AdapterAdd {
+  const uint4* u[kAddRows];
+  uint4 w[kAddRows][2];
+  __device__ __forceinline__ void rows(const Args& a, int64_t p, int step, int64_t end, int o) {
 #pragma unroll
-  for (int r = 0; r < kAdd; r += 4) {
-    const uint4* u[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t q = p + static_cast<int64_t>(step) * (r + j);
+    for (int j = 0; j < kAddRows; ++j) {
+      const int64_t q = p + static_cast<int64_t>(step) * j;
       const int ad = q < end && o < a.O ? a.adapter[q] : -1;
       u[j] = ad >= 0 && ad < a.L ? reinterpret_cast<const uint4*>(a.up + (static_cast<int64_t>(ad) * a.O + o) * a.D)
                                  : nullptr;
-      add[r + j] = 0.0f;
     }
-    if (p + static_cast<int64_t>(step) * r >= end) continue;
-    for (int d = 0; d < a.D / 8; d += 2) {
-      uint4 w[4][2];
+  }
+  __device__ __forceinline__ void fetch(int d, int n) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < kAddRows; ++j)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (u[j] != nullptr && d + h < a.D / 8) w[j][h] = u[j][d + h];
+      for (int h = 0; h < 2; ++h)
+        if (u[j] != nullptr && d + h < n) w[j][h] = u[j][d + h];
+  }
+  __device__ __forceinline__ void sum(int d, int D, const float* low, float* add) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (u[j] == nullptr) continue;
-        float s = add[r + j];
+    for (int j = 0; j < kAddRows; ++j) {
+      if (u[j] == nullptr) continue;
+      float s = add[j];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (d + h >= D / 8) continue;
+        const float4* l = reinterpret_cast<const float4*>(low + j * D + 8 * (d + h));
+        const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&w[j][h]);
+        const float4 l0 = l[0], l1 = l[1];
+        const float2 f0 = __bfloat1622float2(b[0]), f1 = __bfloat1622float2(b[1]), f2 = __bfloat1622float2(b[2]),
+                     f3 = __bfloat1622float2(b[3]);
+        s = fmaf(f0.x, l0.x, s);
+        s = fmaf(f0.y, l0.y, s);
+        s = fmaf(f1.x, l0.z, s);
+        s = fmaf(f1.y, l0.w, s);
+        s = fmaf(f2.x, l1.x, s);
+        s = fmaf(f2.y, l1.y, s);
+        s = fmaf(f3.x, l1.z, s);
+        s = fmaf(f3.y, l1.w, s);
+      }
+      add[j] = s;
+    }
+  }
+};
+
+// low[q][d] = scale (down[d] x) for this CTA's rows, by its four epilogue warps: where
+// the rows are so few that a launch of its own costs more
+__device__ __forceinline__ void own_low(const Args& a, int64_t p, int step, int64_t end, float* low) {
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - 2;
+  constexpr int kDeep = 4;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  for (int q = 0; q < kAdd && p + static_cast<int64_t>(step) * q < end; ++q) {
+    const int64_t row = p + static_cast<int64_t>(step) * q;
+    const int ad = a.adapter[row];
+    if (ad < 0 || ad >= a.L) continue;
+    const float scale = a.scale != nullptr ? a.scale[ad] : 1.0f;
+    const uint4* x = reinterpret_cast<const uint4*>(a.x + row * a.K);
+    for (int d = warp * kDeep; d < a.D; d += 4 * kDeep) {  // D is a multiple of 8
+      const uint4* w = reinterpret_cast<const uint4*>(a.down + (static_cast<int64_t>(ad) * a.D + d) * a.K);
+      const int n = a.K / 8;
+      float s[kDeep] = {};
+      for (int v0 = lane; v0 < n; v0 += 64) {
+        uint4 xv[2], wv[2][kDeep];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (d + h >= a.D / 8) continue;
-          const float* l = low + (r + j) * a.D + 8 * (d + h);
-          const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&w[j][h]);
+          const bool in = v0 + 32 * h < n;
+          xv[h] = in ? x[v0 + 32 * h] : zero;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = __bfloat1622float2(b[e]);
-            s = fmaf(f.x, l[2 * e], s);
-            s = fmaf(f.y, l[2 * e + 1], s);
+          for (int e = 0; e < kDeep; ++e) wv[h][e] = in ? w[static_cast<int64_t>(e) * n + v0 + 32 * h] : zero;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (v0 + 32 * h >= n) continue;
+          const __nv_bfloat162* xb = reinterpret_cast<const __nv_bfloat162*>(&xv[h]);
+#pragma unroll
+          for (int e = 0; e < kDeep; ++e) {
+            const __nv_bfloat162* wb = reinterpret_cast<const __nv_bfloat162*>(&wv[h][e]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = __bfloat1622float2(xb[i]), g = __bfloat1622float2(wb[i]);
+              s[e] = fmaf(f.x, g.x, s[e]);
+              s[e] = fmaf(f.y, g.y, s[e]);
+            }
           }
         }
-        add[r + j] = s;
+      }
+#pragma unroll
+      for (int e = 0; e < kDeep; ++e) {
+#pragma unroll
+        for (int m = 16; m > 0; m >>= 1) s[e] += __shfl_xor_sync(0xffffffffu, s[e], m);
+        if (lane == e) low[q * a.D + d + e] = scale * s[e];
       }
     }
   }
@@ -204,7 +262,7 @@ __device__ __forceinline__ void ld_cols(float (&v)[16], uint32_t taddr) {
 // grid: x = tiles of 128 outputs x split (a cluster along x), y = groups that
 // have rows, z = row tiles that start apart.
 template <int kN, int kEpi>
-__global__ void __launch_bounds__(kThreads) thin_kernel(const __grid_constant__ CUtensorMap mw,
+__global__ void __launch_bounds__(kThreads, 2) thin_kernel(const __grid_constant__ CUtensorMap mw,
                                                         const __grid_constant__ CUtensorMap mx, const Args a) {
   using Sh = Shape<kN>;
   constexpr int S = Sh::kStages;
@@ -301,14 +359,33 @@ __global__ void __launch_bounds__(kThreads) thin_kernel(const __grid_constant__ 
     const int rows = r1 - p < kN ? static_cast<int>(r1 - p) : kN;
     if (warp >= 2) {
       if (kEpi == kAdapter) {  // while the weights arrive
-        wait_previous();       // low_rank
         float* low = reinterpret_cast<float*>(ring + S * Sh::kStage + sizeof(Control));
         const int64_t end = r1 < p + kN ? r1 : p + kN;
+        AdapterAdd f;
+        f.rows(a, p + rank, split, end, o);
+        f.fetch(0, a.D / 8);
+        wait_previous();
         named_sync(1, 128);  // the last row tile's are no longer read
-        for (int q = 0; q < kAdd && p + rank + q * split < end; ++q)
-          for (int d = tid - 64; d < a.D; d += 128) low[q * a.D + d] = a.low_rank[(p + rank + q * split) * a.D + d];
+        if (a.low_rank == nullptr)
+          own_low(a, p + rank, split, end, low);
+        else
+          for (int q = 0; q < kAdd && p + rank + q * split < end; ++q)
+            for (int d = tid - 64; d < a.D; d += 128) low[q * a.D + d] = a.low_rank[(p + rank + q * split) * a.D + d];
         named_sync(1, 128);
-        adapter_add(a, p + rank, split, end, o, low, add);
+#pragma unroll
+        for (int j = 0; j < kAdd; ++j) add[j] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kAdd; j += kAddRows) {
+          if (p + rank + j * split >= end) break;
+          if (j > 0) {
+            f.rows(a, p + rank + j * split, split, end, o);
+            f.fetch(0, a.D / 8);
+          }
+          for (int d = 0; d < a.D / 8; d += 2) {
+            f.sum(d, a.D, low + j * a.D, add + j);
+            f.fetch(d + 2, a.D / 8);
+          }
+        }
       }
       if (k1 > k0) ok = tc::warp_wait(&c.acc, static_cast<uint32_t>(it & 1)) && ok;
       tc::fence_after();
