@@ -46,19 +46,21 @@ template <int kCG, int kBN, bool kAMN, bool kBMN, bool kWGrad, int kEpi>
 int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2, const Args& a, cudaStream_t s) {
   using Sh = Shape<kCG, kBN, kEpi>;
   if (!tma::bind_context()) return camoe::tm::status(cudaErrorNoDevice);
-  CUtensorMap m[4];
+  CUtensorMap m[6];
   const int ra = kAMN ? 64 : 128, rb = Sh::box(kBMN);
   bool ok = tma::encode_3d_sw128(&m[0], A.base, A.inner, A.rows, A.depth, ra) &&
             tma::encode_3d_sw128(&m[1], B.base, B.inner, B.rows, B.depth, rb);
-  if (kEpi == kDRelu2)  // A2: h, B2: low, in the epilogue's boxes of 32 rows
-    ok = ok && tma::encode_2d_rows(&m[2], A2.base, 2 * A2.inner, A2.rows, 64, 32) &&
-         (a.low == nullptr || tma::encode_2d_rows(&m[3], a.low, low_stride(a.N), a.R, 32, 32));
+  m[2] = m[4] = m[5] = m[0], m[3] = m[1];  // where a kernel has no use for them
+  if (kEpi == kDRelu2)  // A2: h
+    ok = ok && tma::encode_2d_rows(&m[2], A2.base, 2 * A2.inner, A2.rows, 64, 32);
   else if (a.K2 > 0)
     ok = ok && tma::encode_3d_sw128(&m[2], A2.base, A2.inner, A2.rows, A2.depth, ra) &&
          tma::encode_3d_sw128(&m[3], B2.base, B2.inner, B2.rows, B2.depth, rb);
-  else
-    m[2] = m[0], m[3] = m[1];
-  if (kEpi == kDRelu2 && a.low == nullptr) m[3] = m[2];
+  // the epilogue's boxes of 32 x 32
+  if (a.scatter == nullptr)
+    ok = ok && tma::encode_2d_rows(&m[4], a.out, 2 * static_cast<int64_t>(a.N),
+                                   kWGrad ? static_cast<int64_t>(a.groups) * a.M : a.R, 64, 32);
+  if (a.low != nullptr) ok = ok && tma::encode_2d_rows(&m[5], a.low, low_stride(a.N), a.R, 32, 32);
   if (!ok) return camoe::tm::status(cudaErrorInvalidValue);
   const int64_t nt = (a.N + kBN - 1) / kBN;
   const int64_t rt = kWGrad ? static_cast<int64_t>(a.groups) * ((a.M + Sh::kBM - 1) / Sh::kBM)
@@ -84,7 +86,7 @@ int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2,
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = kCG > 1 ? 2 : 1;
-  return camoe::tm::status(cudaLaunchKernelEx(&cfg, kernel, m[0], m[1], m[2], m[3], a));
+  return camoe::tm::status(cudaLaunchKernelEx(&cfg, kernel, m[0], m[1], m[2], m[3], m[4], m[5], a));
 }
 
 }  // namespace tc
