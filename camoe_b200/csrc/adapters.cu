@@ -8,12 +8,12 @@
 // runs), to whose sums each output adds its row of up times low, in fp32, before
 // the one rounding.
 //
-// Many rows (prompts): the rows are sorted by adapter, low = scale (xs down^T)
-// is one grouped product (rounded to bf16, the type of the next product's
-// operand), and the projection is a grouped product over the same sorted rows
-// whose sum runs over [x | low] against [weight | up[a]]: the adapter is D more
-// columns of K in the tensor cores, its bytes are read once per row tile, and
-// the result goes to the row that it came from.
+// Many rows (prompts): the rows are sorted by adapter, low = scale (xs down^T) is one
+// grouped product (rounded to bf16, the type of the next product's operand), and
+// the projection's sum runs over [x | low] against [weight | up[a]]: an adapter is
+// D more columns of k for the row tiles that hold rows of it, with zeros in the
+// other rows of the tile (kBlocks and kJoined in tc_gemm.cuh), so row tiles are
+// full whatever the adapters' shares.  The result goes to the row that it came from.
 #include "camoe_experts.h"
 #include "tc_launch.cuh"
 
@@ -76,9 +76,12 @@ __global__ void __launch_bounds__(kThreads) low_kernel(const bf16* __restrict__ 
   if (lane == 0) low[static_cast<int64_t>(n) * D + d] = scale != nullptr ? scale[a] * s : s;
 }
 
-// Rows that are streamed rather than sorted: a few, or so few per adapter that
-// row tiles of one adapter each would be mostly empty.
-bool few_rows(int64_t N, int64_t L) { return N <= 256 || N < 16 * L; }
+// Rows that are streamed rather than sorted: few, and with little of the adapters' own
+// work, which each row does for itself there.  B200, us streamed / in tiles, rows
+// that mix L adapters, N x C x M x D, L:  128 x 2048 x 2048 x 32, 64: 19 / 53;
+// 256 x 2048 x 2048 x 32, 64: 30 / 58;  384: 49 / 49;  512 x 1024 x 1024 x 16, 12:
+// 23 / 25;  512 x 1024 x 1024 x 64, 3: 51 / 23;  256 x 2048 x 4096 x 128, 64: 132 / 78.
+bool few_rows(int64_t N, int64_t M, int64_t D) { return N <= 128 || (N <= 512 && N * M * D <= (24 << 20)); }
 
 // A few rows whose low-rank parts are little work for each CTA of a cluster of four
 // (64 KB of down read at most): every tile of the projection works them out for
@@ -88,13 +91,16 @@ bool own_low(int64_t N, int64_t C, int64_t D) { return N <= 8 && (N + 3) / 4 * C
 
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 
+constexpr int64_t kTile = 256;  // rows of a tile
+int64_t blocks(int64_t N, int64_t L) { return tc::most_blocks(N, L, kTile); }
+
 struct Layout {  // of the workspace
   size_t low, xs, offsets, position, source, sort, total;
 };
-Layout layout(int64_t N, int64_t C, int64_t D, int64_t L) {
+Layout layout(int64_t N, int64_t C, int64_t M, int64_t D, int64_t L) {
   Layout w{};
   const size_t n = static_cast<size_t>(N);
-  if (few_rows(N, L)) {
+  if (few_rows(N, M, D)) {
     w.total = up16(n * static_cast<size_t>(D) * sizeof(float));
     return w;
   }
@@ -104,7 +110,7 @@ Layout layout(int64_t N, int64_t C, int64_t D, int64_t L) {
     at += up16(bytes);
     return here;
   };
-  w.low = take(n * static_cast<size_t>(D) * sizeof(bf16));
+  w.low = take(static_cast<size_t>(blocks(N, L)) * kTile * static_cast<size_t>(D) * sizeof(bf16));
   w.xs = take(n * static_cast<size_t>(C) * sizeof(bf16));
   w.offsets = take(static_cast<size_t>(L + 2) * sizeof(int));
   w.position = take(n * sizeof(int));
@@ -123,7 +129,7 @@ int check(int64_t N, int64_t C, int64_t M, int64_t D, int64_t L) {
 
 template <int kBN>
 int low_product(const bf16* xs, const void* down, const tc::Args& a, int64_t L, cudaStream_t st) {
-  return tc::launch<1, kBN, false, false, false, tc::kScale>({xs, a.K, a.R, 1}, {down, a.K, a.N, L}, {}, {}, a, st);
+  return tc::launch<2, kBN, false, false, tc::kBlocks, tc::kScale>({xs, a.K, a.R, 1}, {down, a.K, a.N, L}, {}, {}, a, st);
 }
 
 }  // namespace adapt
@@ -132,7 +138,7 @@ int low_product(const bf16* xs, const void* down, const tc::Args& a, int64_t L, 
 extern "C" {
 
 size_t camoe_ad_work_bytes(int64_t N, int64_t C, int64_t M, int64_t D, int64_t L) {
-  return camoe::adapt::check(N, C, M, D, L) == 0 ? camoe::adapt::layout(N, C, D, L).total : 0;
+  return camoe::adapt::check(N, C, M, D, L) == 0 ? camoe::adapt::layout(N, C, M, D, L).total : 0;
 }
 
 int camoe_ad_linear(const void* x, const void* weight, const void* down, const void* up, const int32_t* adapter,
@@ -147,21 +153,18 @@ int camoe_ad_linear(const void* x, const void* weight, const void* down, const v
     if (p == nullptr) return 1;
   for (const void* p : {x, weight, down, up, static_cast<const void*>(y), static_cast<const void*>(work)})
     if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0) return 4;
-  const Layout w = layout(N, C, D, L);
+  const Layout w = layout(N, C, M, D, L);
   if (work_bytes < w.total) return 5;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   unsigned char* base = static_cast<unsigned char*>(work);
   const int c = static_cast<int>(C), m = static_cast<int>(M), d = static_cast<int>(D), l = static_cast<int>(L);
   const bf16* xb = static_cast<const bf16*>(x);
-  if (few_rows(N, L)) {
+  if (few_rows(N, M, D)) {
     float* low = static_cast<float*>(work);
     const bool own = own_low(N, C, D);
     if (!own) {
-      for (int64_t n0 = 0; n0 < N; n0 += 32768) {  // grid.y holds 65535
-        const int64_t n = N - n0 < 32768 ? N - n0 : 32768;
-        low_kernel<<<dim3((d + 7) / 8, static_cast<unsigned>(n)), kThreads, 0, s>>>(
-            xb + n0 * C, static_cast<const bf16*>(down), adapter + n0, scale, low + n0 * D, c, d, l);
-      }
+      low_kernel<<<dim3((d + 7) / 8, static_cast<unsigned>(N)), kThreads, 0, s>>>(
+          xb, static_cast<const bf16*>(down), adapter, scale, low, c, d, l);
       if (const int st = camoe::tm::status(cudaGetLastError())) return st;
     }
     thin::Args t{};
@@ -202,16 +205,13 @@ int camoe_ad_linear(const void* x, const void* weight, const void* down, const v
   const int st = D <= 64 ? low_product<64>(xs, down, a, L, s)
                          : (D <= 128 ? low_product<128>(xs, down, a, L, s) : low_product<256>(xs, down, a, L, s));
   if (st != 0) return st;
-  a.groups = l + 1;
   a.N = m;
   a.K2 = d;
-  a.groups2 = l;
-  a.b_shared = 1;
   a.out = static_cast<bf16*>(y);
   a.scale = nullptr;
   a.scatter = source;
-  return tc::launch<2, 256, false, false, false, tc::kPlain>({xs, C, N, 1}, {weight, C, M, 1}, {low, D, N, 1},
-                                                             {up, D, M, L}, a, s);
+  return tc::launch<2, 256, false, false, tc::kJoined, tc::kPlain>(
+      {xs, C, N, 1}, {weight, C, M, 1}, {low, D, blocks(N, L) * kTile, 1}, {up, D, M, L}, a, s);
 }
 
 }  // extern "C"

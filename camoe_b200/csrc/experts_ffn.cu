@@ -73,7 +73,7 @@ tc::Args args(const int* offsets, int64_t E, int64_t R, int64_t N, int64_t K, vo
 template <bool kBMN, int kEpi>
 int rows_product(const void* x, const void* w, const tc::Args& a, int64_t E, cudaStream_t st,
                  const void* h = nullptr) {
-  return tc::launch<2, 256, false, kBMN, false, kEpi>(
+  return tc::launch<2, 256, false, kBMN, tc::kRows, kEpi>(
       {x, a.K, a.R, 1}, kBMN ? tc::Matrix{w, a.N, a.K, E} : tc::Matrix{w, a.K, a.N, E}, {h, a.N, a.R, 1},
       {}, a, st);
 }
@@ -153,13 +153,13 @@ int camoe_ex_ffn_bwd(const void* dys, const void* xs, const void* w_up, const vo
     if (xs == nullptr) return 1;
     tc::Args a = args(offsets, E, R, C, 0, dw_up);
     a.M = static_cast<int>(F);
-    if (const int st = tc::launch<2, 256, true, true, true, tc::kPlain>({dpre, F, R, 1}, {xs, C, R, 1}, {}, {}, a, s))
+    if (const int st = tc::launch<2, 256, true, true, tc::kWeights, tc::kPlain>({dpre, F, R, 1}, {xs, C, R, 1}, {}, {}, a, s))
       return st;
   }
   if (dw_down != nullptr) {
     tc::Args a = args(offsets, E, R, F, 0, dw_down);
     a.M = static_cast<int>(C);
-    return tc::launch<2, 256, true, true, true, tc::kPlain>({dys, C, R, 1}, {h, F, R, 1}, {}, {}, a, s);
+    return tc::launch<2, 256, true, true, tc::kWeights, tc::kPlain>({dys, C, R, 1}, {h, F, R, 1}, {}, {}, a, s);
   }
   return 0;
 }

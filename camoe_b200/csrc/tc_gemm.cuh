@@ -1,12 +1,19 @@
 // Products of grouped rows on the 5th-generation tensor cores (tcgen05): one
 // kernel for the experts' six products and the adapters' two.
 //
-// Rows: for the rows p of group g (p in [offsets[g], offsets[g + 1]))
-//     out[p][n] = sum over k of A[p][k] B_g[n][k]  (+ a second pair A2, B2_g)
+// kRows: for the rows p of group g (p in [offsets[g], offsets[g + 1]))
+//     out[p][n] = sum over k of A[p][k] B_g[n][k]
 //   A's rows have k contiguous; B_g is stored [N][K] (k contiguous) or [K][N]
 //   (n contiguous), which is a bit of the instruction descriptor.
-// Weight gradients: out_g[m][n] = sum over the rows p of g of A[p][m] B[p][n],
-//   both stored with m or n contiguous.
+// kWeights (weight gradients): out_g[m][n] = sum over the rows p of g of
+//   A[p][m] B[p][n], both stored with m or n contiguous.
+// kBlocks and kJoined (adapters), over row tiles of the whole array, which the
+//   groups' rows cut as they may:
+//   kBlocks: for each group and row tile that share rows a block of the tile's
+//     rows with the group's product in its own rows and zeros in the others;
+//   kJoined: out[p][n] = sum over k of A[p][k] B[n][k] + sum over the groups g of
+//     p's tile of sum over d of block[p][d] B2_g[n][d]: a group's product reaches
+//     its own rows only, as more of the same sum.
 //
 // One CTA (or a pair of CTAs on two SMs, kCG = 2) per tile of 128 kCG rows x kBN
 // columns, persistent over the tiles:
@@ -44,6 +51,7 @@ constexpr int kMaxGroups = 1025;  // 1024 and the rows of no group
 constexpr int kRingBytes = 192 * 1024;
 constexpr uint32_t kBox = 64 * 128;  // a box of 64 columns x 64 rows
 
+enum Mode : int { kRows = 0, kWeights = 1, kBlocks = 2, kJoined = 3 };
 enum Epilogue : int {
   kPlain = 0,   // out = acc
   kRelu2 = 1,   // out = relu(acc)^2
@@ -59,8 +67,7 @@ struct Args {
   int groups;
   int64_t R;             // rows of A (the sorted arrays)
   int M, N, K;           // M: weight gradients only
-  int K2, groups2;       // depth of the second pair, which groups below groups2 have
-  int b_shared;          // B is one matrix for all groups
+  int K2;                // kJoined: depth of the blocks (maps ma2: blocks, mb2: B2)
   int zero_tail;         // write zeros to the rows behind the last group
   bf16* out;
   int8_t* low;           // [R, low_stride(N)] (kRelu2, kDRelu2) or null: the 8 bits of the value below bf16's
@@ -90,6 +97,7 @@ struct Control {
   uint64_t full[10], empty[10], tail[10], peer_tail[10], acc_full[2], acc_empty[2], drained, aux[kEpiWarps][2];
   uint32_t tmem;
   int tiles[kMaxGroups + 1];  // row tiles of the groups before each
+  int first[kMaxGroups + 1];  // the groups' first rows, clamped to R
 };
 
 template <int kCG, int kBN, int kEpi>
@@ -277,9 +285,11 @@ struct Tile {
   int64_t row0, row1;  // the group's rows from the tile's first (weight gradients: all of the group's)
   int m0;              // weight gradients: first output row
   int nk1, nk;         // pieces of the first pair, of both
+  int tile;            // kBlocks: block; kJoined: row tile
+  int64_t lead;        // kBlocks: rows of the tile before the group's
 };
 
-template <int kCG, int kBN, bool kWGrad>
+template <int kCG, int kBN, int kMode>
 struct Tiles {
   const Args& a;
   const Control& c;
@@ -287,8 +297,10 @@ struct Tiles {
   int whole, jobs;  // tiles done whole, and these with the halves of the others
   __device__ Tiles(const Args& args, const Control& ctl) : a(args), c(ctl) {
     nt = (a.N + kBN - 1) / kBN;
-    mt = kWGrad ? (a.M + (128 * kCG) - 1) / (128 * kCG) : 0;
-    const int total = kWGrad ? a.groups * mt * nt : c.tiles[a.groups] * nt;
+    mt = kMode == kWeights ? (a.M + (128 * kCG) - 1) / (128 * kCG) : 0;
+    const int total = kMode == kWeights ? a.groups * mt * nt
+                      : kMode == kJoined ? static_cast<int>((a.R + 128 * kCG - 1) / (128 * kCG)) * nt
+                                         : c.tiles[a.groups] * nt;
     // Tiles left for a last round that would leave half of the workers or more
     // without one are done as halves of kBN / 2 columns, which take half the time.
     const int workers = gridDim.x / kCG, left = total % workers;
@@ -296,10 +308,20 @@ struct Tiles {
     whole = halves ? total - left : total;
     jobs = halves ? whole + 2 * left : total;
   }
-  // rows are clamped to R: whatever the offsets hold, nothing outside the arrays is touched
-  __device__ int64_t first(int g) const {
-    const int64_t o = a.offsets[g];
-    return o < 0 ? 0 : (o < a.R ? o : a.R);
+  __device__ int64_t first(int g) const { return c.first[g]; }
+  // kJoined: the first group at or behind g with rows of the row tile, `groups` if none
+  __device__ int next_group(int g, int tile) const {
+    const int64_t end = static_cast<int64_t>(tile + 1) * (128 * kCG);
+    while (g < a.groups && c.first[g + 1] <= c.first[g]) ++g;
+    return g < a.groups && c.first[g] < end ? g : a.groups;
+  }
+  __device__ int group_at(int64_t row) const {  // the last group that starts at or before the row
+    int lo = 0, hi = a.groups;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (c.first[mid] <= row) lo = mid; else hi = mid;
+    }
+    return lo;
   }
   __device__ Tile get(int job) const {
     Tile x;
@@ -307,12 +329,22 @@ struct Tiles {
     const int rt = t / nt;
     x.width = job < whole ? kBN : kBN / 2;
     x.n0 = (t - rt * nt) * kBN + (job < whole ? 0 : (job - whole) % 2 * (kBN / 2));
-    if (kWGrad) {
+    if (kMode == kWeights) {
       x.group = rt / mt;
       x.m0 = (rt - x.group * mt) * (128 * kCG);
       x.row0 = first(x.group);
       x.row1 = first(x.group + 1);
       x.nk1 = x.nk = x.row1 > x.row0 ? static_cast<int>((x.row1 - x.row0 + kBK - 1) / kBK) : 0;
+    } else if (kMode == kJoined) {
+      x.group = group_at(static_cast<int64_t>(rt) * (128 * kCG));
+      if (c.first[x.group + 1] <= static_cast<int64_t>(rt) * (128 * kCG)) ++x.group;  // ends before the tile
+      x.m0 = 0;
+      x.tile = rt;
+      x.row0 = static_cast<int64_t>(rt) * (128 * kCG);
+      x.row1 = a.R;
+      x.nk1 = x.nk = (a.K + kBK - 1) / kBK;
+      const int each = (a.K2 + kBK - 1) / kBK;
+      for (int g = next_group(x.group, rt); g < a.groups; g = next_group(g + 1, rt)) x.nk += each;
     } else {
       int lo = 0, hi = a.groups;  // the last group whose first row tile is at most rt
       while (hi - lo > 1) {
@@ -321,10 +353,14 @@ struct Tiles {
       }
       x.group = lo;
       x.m0 = 0;
+      x.tile = rt;
       x.row0 = first(lo) + static_cast<int64_t>(rt - c.tiles[lo]) * (128 * kCG);
       x.row1 = first(lo + 1);
-      x.nk1 = (a.K + kBK - 1) / kBK;
-      x.nk = x.nk1 + (lo < a.groups2 ? (a.K2 + kBK - 1) / kBK : 0);
+      if (kMode == kBlocks) {
+        x.row0 = (first(lo) / (128 * kCG) + rt - c.tiles[lo]) * (128 * kCG);
+        x.lead = first(lo) - x.row0;
+      }
+      x.nk1 = x.nk = (a.K + kBK - 1) / kBK;
     }
     return x;
   }
@@ -360,7 +396,7 @@ __device__ __forceinline__ float finish(float x, float aux, float scale) {
 __device__ __forceinline__ uint32_t out_at(int r, int q) { return r * 64 + ((q ^ ((r >> 1) & 3)) << 4); }
 __device__ __forceinline__ uint32_t low_at(int r, int q) { return r * 32 + ((q ^ ((r >> 2) & 1)) << 4); }
 
-template <int kCG, int kBN, bool kAMN, bool kBMN, bool kWGrad, int kEpi>
+template <int kCG, int kBN, bool kAMN, bool kBMN, int kMode, int kEpi>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
                 const __grid_constant__ CUtensorMap ma2, const __grid_constant__ CUtensorMap mb2,
@@ -400,16 +436,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   // (programmatic dependent launch); what follows reads what that one wrote.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!kWGrad && warp == 2) {  // row tiles of each group
+  if (warp == 2) {  // the groups' first rows and row tiles
+    // rows are clamped to R: whatever the offsets hold, nothing outside the arrays is touched
+    const auto clamped = [&](int g) {
+      const int64_t o = a.offsets[g];
+      return o < 0 ? 0 : (o < a.R ? o : a.R);
+    };
     int carry = 0;
     for (int g0 = 0; g0 < a.groups; g0 += 32) {
       const int g = g0 + lane;
       int n = 0;
       if (g < a.groups) {
-        int64_t r0 = a.offsets[g], r1 = a.offsets[g + 1];
-        r0 = r0 < 0 ? 0 : (r0 < a.R ? r0 : a.R);
-        r1 = r1 < 0 ? 0 : (r1 < a.R ? r1 : a.R);
-        n = r1 > r0 ? static_cast<int>((r1 - r0 + Sh::kBM - 1) / Sh::kBM) : 0;
+        const int64_t r0 = clamped(g), r1 = clamped(g + 1);
+        if (r1 > r0)
+          n = kMode == kRows ? static_cast<int>((r1 - r0 + Sh::kBM - 1) / Sh::kBM)
+                             : static_cast<int>((r1 - 1) / Sh::kBM - r0 / Sh::kBM + 1);
+        c.first[g] = static_cast<int>(r0);
       }
       int x = n;
 #pragma unroll
@@ -420,14 +462,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (g < a.groups) c.tiles[g] = carry + x - n;
       carry += __shfl_sync(0xffffffffu, x, 31);
     }
-    if (lane == 0) c.tiles[a.groups] = carry;
+    if (lane == 0) {
+      c.tiles[a.groups] = carry;
+      c.first[a.groups] = static_cast<int>(clamped(a.groups));
+    }
   }
   fence_before();
   __syncthreads();
   if (kCG > 1) pair_sync<kCG>();
   fence_after();
   const uint32_t tmem = c.tmem, ring0 = sm_addr(ring);
-  const Tiles<kCG, kBN, kWGrad> tiles(a, c);
+  const Tiles<kCG, kBN, kMode> tiles(a, c);
 
   // Producer and product issue run as whole warps of which an elected lane acts: with
   // the operands uniform over the warp the issue is short (a branch on the lane
@@ -444,9 +489,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool two = x.width / kCG > kBBox;  // boxes of B beyond the first
       const int boxes = x.width / kCG / kBBox;
       const uint32_t bytes = Sh::kABytes + static_cast<uint32_t>(x.width / kCG) * 128u;
-      const bool cut = kWGrad && ((x.row1 - x.row0) % kBK) != 0;
+      const bool cut = kMode == kWeights && ((x.row1 - x.row0) % kBK) != 0;
+      const int each = (a.K2 + kBK - 1) / kBK;
+      int part = 0, group = 0, block = 0;  // kJoined
       for (int j = 0; j < x.nk; ++j) {
         if (round > 0 && !(ok = warp_wait(&c.empty[s], (round - 1) & 1u))) break;
+        if (kMode == kJoined && j >= x.nk1) {  // the next 64 columns of the group's block, or the next group's
+          if (++part == each || j == x.nk1) {
+            part = 0;
+            group = tiles.next_group(j == x.nk1 ? x.group : group + 1, x.tile);
+            block = (c.tiles[group] + x.tile - c.first[group] / Sh::kBM) * Sh::kBM;
+          }
+        }
         if (elect_one()) {
           const bool last = cut && j == x.nk - 1;
           // a piece to be cleared lands on this CTA's own barrier
@@ -456,19 +510,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           else if (rank == 0)  // for both CTAs: the pair's loads complete on the leader's barrier
             mbar_arrive_expect_tx(&c.full[s], kCG * bytes);
           const uint32_t sa = ring0 + s * kStage, sb = sa + Sh::kABytes;
-          if (kWGrad) {
+          if (kMode == kWeights) {
             const int r = static_cast<int>(x.row0) + j * kBK;
             load_box<kCG>(sa, &ma, m, r, 0, bar);
             load_box<kCG>(sa + kBox, &ma, m + 64, r, 0, bar);
             load_box<kCG>(sb, &mb, n, r, 0, bar);
             for (int q = 1; q < boxes; ++q) load_box<kCG>(sb + q * kBox, &mb, n + 64 * q, r, 0, bar);
           } else {
-            const bool one = j < x.nk1;
-            const int k = (one ? j : j - x.nk1) * kBK;
+            const bool one = kMode != kJoined || j < x.nk1;
+            const int k = one ? j * kBK : part * kBK;
             const CUtensorMap* pa = one ? &ma : &ma2;
             const CUtensorMap* pb = one ? &mb : &mb2;
-            const int z = one && a.b_shared ? 0 : x.group;
-            load_box<kCG>(sa, pa, k, row, 0, bar);
+            const int z = kMode == kJoined ? (one ? 0 : group) : x.group;
+            load_box<kCG>(sa, pa, k, one ? row : block + static_cast<int>(rank) * 128, 0, bar);
             if (kBMN) {
               load_box<kCG>(sb, pb, n, k, z, bar);
               for (int q = 1; q < boxes; ++q) load_box<kCG>(sb + q * kBox, pb, n + 64 * q, k, z, bar);
@@ -494,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int t = worker; ok && t < tiles.jobs; t += workers) {
       const Tile x = tiles.get(t);
-      const int tail = kWGrad ? static_cast<int>((x.row1 - x.row0) % kBK) : 0;
+      const int tail = kMode == kWeights ? static_cast<int>((x.row1 - x.row0) % kBK) : 0;
       if (x.nk == 0) continue;
       const uint32_t idesc = x.width == kBN ? instr<kAMN, kBMN>(Sh::kBM, kBN) : instr<kAMN, kBMN>(Sh::kBM, kBN / 2);
       const int boxes = static_cast<int>((Sh::kABytes + static_cast<uint32_t>(x.width / kCG) * 128u) / kBox);
@@ -505,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int j = 0; j < x.nk; ++j) {
         const uint32_t sa = ring0 + s * kStage;
-        if (kWGrad && tail != 0 && j == x.nk - 1) {
+        if (kMode == kWeights && tail != 0 && j == x.nk - 1) {
           if (!(ok = warp_wait(&c.tail[s], (tail_phase >> s) & 1u))) break;
           tail_phase ^= 1u << s;
 #pragma unroll 1
@@ -569,12 +623,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool have = x.nk > 0;
       // the warp's 32 rows: the first, and how many of them exist
       const int in_tile = static_cast<int>(rank) * 128 + 32 * quarter;
-      const int64_t row0 = (kWGrad ? static_cast<int64_t>(x.group) * a.M + x.m0 : x.row0) + in_tile;
-      const int64_t left = (kWGrad ? a.M - x.m0 : x.row1 - x.row0) - in_tile;
+      const int64_t row0 = (kMode == kWeights  ? static_cast<int64_t>(x.group) * a.M + x.m0
+                            : kMode == kBlocks ? static_cast<int64_t>(x.tile) * Sh::kBM
+                                               : x.row0) + in_tile;
+      const int64_t left = (kMode == kWeights ? a.M - x.m0 : kMode == kBlocks ? Sh::kBM : x.row1 - x.row0) - in_tile;
+      // kBlocks: this lane's row is the group's
+      const bool live = kMode != kBlocks || (in_tile + lane >= x.lead && x.row0 + in_tile + lane < x.row1);
       const int rows = left < 32 ? (left > 0 ? static_cast<int>(left) : 0) : 32;
       const float scale = kEpi == kScale && a.scale != nullptr ? a.scale[x.group] : 1.0f;
       int to = 0;  // where this lane's row goes
-      if (!kWGrad && a.scatter != nullptr && lane < rows) to = a.scatter[row0 + lane];
+      if (kMode != kWeights && a.scatter != nullptr && lane < rows) to = a.scatter[row0 + lane];
       const int begin = half * (x.width / 2), end = begin + x.width / 2;
       const int cols = a.N - x.n0 < end ? a.N - x.n0 : end;
       if (kEpi == kDRelu2 && rows > 0 && begin < cols) {
@@ -599,6 +657,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 32; ++e) v[e] = 0u;
         }
         if (rows == 0) continue;  // the whole warp
+        if (!live) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0u;
+        }
         unsigned char* out = outs;
         unsigned char* lows = all_lows;
         if (kEpi == kDRelu2) {  // h lies where the result will be staged
@@ -658,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Whole boxes of 32 rows go out by TMA; with loads and stores through registers
         // in its place kDRelu2 took 127 us against 122 for 16384 rows x 1024 x 4096 (the
         // others within 1 us).
-        if (rows == 32 && (kWGrad || a.scatter == nullptr)) {
+        if (rows == 32 && (kMode == kWeights || a.scatter == nullptr)) {
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
@@ -673,7 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = 8 * i + (lane >> 2), m = n + 8 * (lane & 3);
-          const int64_t dst = !kWGrad && a.scatter != nullptr ? __shfl_sync(0xffffffffu, to, r) : row0 + r;
+          const int64_t dst = kMode != kWeights && a.scatter != nullptr ? __shfl_sync(0xffffffffu, to, r) : row0 + r;
           if (r < rows && m < a.N)
             *reinterpret_cast<uint4*>(a.out + dst * a.N + m) =
                 *reinterpret_cast<const uint4*>(out + out_at(r, lane & 3));
@@ -695,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) bulk_wait_all();
     for (; !ok && steps < asked; ++steps)  // as above: the copies in flight end first
       mbar_wait(&c.aux[ew][steps & 1], static_cast<uint32_t>((steps >> 1) & 1));
-    if (!kWGrad && a.zero_tail) {
+    if (kMode != kWeights && a.zero_tail) {
       const int64_t pieces = a.N / 8;
       const int64_t end = a.R * pieces;
       uint4* out = reinterpret_cast<uint4*>(a.out);

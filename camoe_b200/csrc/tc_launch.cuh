@@ -19,6 +19,11 @@ struct Matrix {
   int64_t inner = 0, rows = 0, depth = 0;
 };
 
+// kBlocks: pairs of a group and a row tile at most
+inline int64_t most_blocks(int64_t R, int64_t groups, int64_t tile) {
+  return (R + tile - 1) / tile + (R < groups ? R : groups);
+}
+
 inline int sm_count() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
@@ -40,9 +45,9 @@ cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
   return e;
 }
 
-// A, B and (K2 > 0) the second pair.  The box of an operand whose k is contiguous
+// A, B and (kJoined) the second pair.  The box of an operand whose k is contiguous
 // has all its rows of a stage; one whose m or n is contiguous, 64 rows of k.
-template <int kCG, int kBN, bool kAMN, bool kBMN, bool kWGrad, int kEpi>
+template <int kCG, int kBN, bool kAMN, bool kBMN, int kMode, int kEpi>
 int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2, const Args& a, cudaStream_t s) {
   using Sh = Shape<kCG, kBN, kEpi>;
   if (!tma::bind_context()) return camoe::tm::status(cudaErrorNoDevice);
@@ -53,25 +58,30 @@ int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2,
   m[2] = m[4] = m[5] = m[0], m[3] = m[1];  // where a kernel has no use for them
   if (kEpi == kDRelu2)  // A2: h
     ok = ok && tma::encode_2d_rows(&m[2], A2.base, 2 * A2.inner, A2.rows, 64, 32);
-  else if (a.K2 > 0)
+  else if (kMode == kJoined)
     ok = ok && tma::encode_3d_sw128(&m[2], A2.base, A2.inner, A2.rows, A2.depth, ra) &&
          tma::encode_3d_sw128(&m[3], B2.base, B2.inner, B2.rows, B2.depth, rb);
   // the epilogue's boxes of 32 x 32
   if (a.scatter == nullptr)
     ok = ok && tma::encode_2d_rows(&m[4], a.out, 2 * static_cast<int64_t>(a.N),
-                                   kWGrad ? static_cast<int64_t>(a.groups) * a.M : a.R, 64, 32);
+                                   kMode == kWeights  ? static_cast<int64_t>(a.groups) * a.M
+                                   : kMode == kBlocks ? most_blocks(a.R, a.groups, Sh::kBM) * Sh::kBM
+                                                      : a.R, 64, 32);
   if (a.low != nullptr) ok = ok && tma::encode_2d_rows(&m[5], a.low, low_stride(a.N), a.R, 32, 32);
   if (!ok) return camoe::tm::status(cudaErrorInvalidValue);
   const int64_t nt = (a.N + kBN - 1) / kBN;
-  const int64_t rt = kWGrad ? static_cast<int64_t>(a.groups) * ((a.M + Sh::kBM - 1) / Sh::kBM)
-                            : a.R / Sh::kBM + (a.R < a.groups ? a.R : a.groups);
+  const int64_t rt = kMode == kWeights  ? static_cast<int64_t>(a.groups) * ((a.M + Sh::kBM - 1) / Sh::kBM)
+                     : kMode == kJoined ? (a.R + Sh::kBM - 1) / Sh::kBM
+                     : kMode == kBlocks ? most_blocks(a.R, a.groups, Sh::kBM)
+                                        : a.R / Sh::kBM + (a.R < a.groups ? a.R : a.groups);
   if (nt * rt > 0x7fffffffLL) return 3;  // CAMOE_ERR_SHAPE
   int64_t pairs = sm_count() / kCG;
   if (pairs < 1) return camoe::tm::status(cudaErrorNoDevice);
   if (2 * nt * rt < pairs) pairs = nt * rt > 0 ? 2 * nt * rt : 1;  // a tile may be done as two halves
-  const auto kernel = gemm_kernel<kCG, kBN, kAMN, kBMN, kWGrad, kEpi>;
+  const auto kernel = gemm_kernel<kCG, kBN, kAMN, kBMN, kMode, kEpi>;
   static std::atomic<uint64_t> opted{0};
   constexpr int smem = smem_bytes<kCG, kBN, kEpi>();
+  static_assert(smem <= 227 * 1024, "a CTA's shared memory");
   if (const int st = camoe::tm::status(allow_smem(kernel, smem, opted))) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(pairs * kCG));
