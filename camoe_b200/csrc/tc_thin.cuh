@@ -272,7 +272,6 @@ __global__ void __launch_bounds__(kThreads, 2) thin_kernel(const __grid_constant
   Control& c = *reinterpret_cast<Control*>(ring + S * Sh::kStage);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = a.split, rank = static_cast<int>(blockIdx.x) % split, tile = static_cast<int>(blockIdx.x) / split;
-  allow_next();
   if (tid == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mw)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mx)) : "memory");
@@ -284,6 +283,9 @@ __global__ void __launch_bounds__(kThreads, 2) thin_kernel(const __grid_constant
     mbar_fence_init();
   }
   if (!a.second) wait_previous();
+  // Not before this wait: a second kernel reads offsets and weights before its own,
+  // so what comes before the first one has to be done by the time it may start.
+  allow_next();
   if (a.zero_tail && blockIdx.y == 0) {
     const int64_t pieces = a.O / 8, used = a.offsets != nullptr ? a.offsets[a.groups] : a.R;
     uint4* out = reinterpret_cast<uint4*>(a.out);

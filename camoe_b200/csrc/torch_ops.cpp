@@ -49,6 +49,12 @@ Tensor bytes(size_t n, const Tensor& like) {
   return n > 0 ? at::empty({static_cast<int64_t>(n)}, like.options().dtype(torch::kUInt8)) : Tensor();
 }
 
+// a gradient as the kernels take it
+Tensor packed(const Tensor& g) {
+  const Tensor t = g.contiguous();
+  return aligned({&t}) ? t : t.clone();
+}
+
 // ---- tokens to their experts and back
 
 struct Sorted {
@@ -86,7 +92,7 @@ struct DispatchFn : torch::autograd::Function<DispatchFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     Tensor dx;
-    if (grads[0].defined()) dx = sum_rows(grads[0].contiguous(), Tensor(), ctx->get_saved_variables()[0]);
+    if (grads[0].defined()) dx = sum_rows(packed(grads[0]), Tensor(), ctx->get_saved_variables()[0]);
     return {dx, Tensor(), Tensor(), Tensor()};
   }
 };
@@ -117,7 +123,7 @@ struct CombineFn : torch::autograd::Function<CombineFn> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &ys = saved[0], &weight = saved[1], &offsets = saved[2], &position = saved[3];
     const c10::cuda::CUDAGuard guard(ys.device());
-    const Tensor dout = grads[0].contiguous();
+    const Tensor dout = packed(grads[0]);
     if (ctx->needs_input_grad(0)) out[0] = at::empty_like(ys);
     if (ctx->needs_input_grad(1)) out[1] = at::empty_like(weight);
     check(camoe_ex_combine_bwd(dout.data_ptr(), dtype_of(ys), ys.data_ptr(), weight.data_ptr<float>(),
@@ -173,7 +179,7 @@ struct FfnFn : torch::autograd::Function<FfnFn> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &xs = saved[0], &w_up = saved[1], &w_down = saved[2], &offsets = saved[3], &h = saved[4];
     const c10::cuda::CUDAGuard guard(xs.device());
-    const Tensor dys = grads[0].contiguous();
+    const Tensor dys = packed(grads[0]);
     for (int i = 0; i < 3; ++i)
       if (ctx->needs_input_grad(i)) out[i] = at::empty_like(saved[i]);
     const Tensor dpre = out[0].defined() || out[1].defined() ? at::empty_like(h) : Tensor();

@@ -53,6 +53,7 @@ CASES = [  # N, C, M, D, L
     (1, 8, 8, 8, 1), (1, 1024, 1024, 16, 4), (7, 200, 72, 24, 3), (9, 64, 136, 40, 2), (33, 2048, 1000, 128, 64),
     (256, 512, 512, 256, 5), (257, 64, 64, 8, 1), (300, 1000, 520, 16, 3), (400, 128, 256, 32, 64),
     (1000, 264, 328, 96, 7), (2100, 512, 1032, 256, 2), (5000, 128, 128, 64, 40),
+    (513, 64, 264, 200, 33), (700, 128, 512, 16, 1024), (3000, 96, 520, 136, 64), (520, 2048, 4096, 64, 12),
 ]
 
 
@@ -61,6 +62,18 @@ def test_adapter_linear(N, C, M, D, L):
     x, w, down, up, adapter, scale = inputs(N, C, M, D, L)
     close(adapters.adapter_linear(x, w, down, up, adapter, scale), exact(x, w, down, up, adapter, scale), 2 * U)
     close(adapters.adapter_linear(x, w, down, up, adapter), exact(x, w, down, up, adapter, None), 2 * U)
+
+
+@pytest.mark.parametrize("lengths", [[256, 256, 256], [1, 255, 257, 0, 511, 1], [0, 0, 700], [600, 0, 0], [255, 1, 0, 768]])
+@pytest.mark.parametrize("none", [0, 100])
+def test_requests_that_end_on_and_beside_tile_borders(lengths, none):
+    L = len(lengths)
+    N = sum(lengths) + none
+    x, w, down, up, _, scale = inputs(N, 128, 320, 72, L, seed=50)
+    adapter = torch.cat([torch.full((n,), a) for a, n in enumerate(lengths)] + [torch.full((none,), -1)])
+    adapter = adapter[torch.randperm(N, generator=torch.Generator().manual_seed(51))] if none else adapter
+    adapter = adapter.to(torch.int32).cuda()
+    close(adapters.adapter_linear(x, w, down, up, adapter, scale), exact(x, w, down, up, adapter, scale), 2 * U)
 
 
 @pytest.mark.parametrize("N", [20, 600])

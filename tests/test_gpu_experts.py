@@ -186,6 +186,9 @@ FFN = [  # counts per expert, unused rows, C, F: rows streamed (few), row tiles'
     ([600, 0, 5, 63, 64, 65], 30, 320, 1000),
     ([0, 0, 700], 0, 1000, 136),
     ([257, 255, 256], 1, 512, 768),
+    ([0] * 300 + [20] + [0] * 700 + [9, 0], 2, 64, 72),         # few rows among 1003 experts
+    ([0] * 12 + [33000 // 30] * 30 + [0] * 3, 0, 64, 136),      # a wide grid of full tiles
+    ([2600, 0, 1700], 10, 256, 264),
 ]
 
 
@@ -332,6 +335,22 @@ def test_the_operators_replay_from_a_cuda_graph(tokens):
         graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, run())
+
+
+def test_gradients_that_are_strided_or_off_alignment():
+    offsets, xs, w_up, w_down = ffn_inputs([40, 20], 0, 64, 128, seed=100)
+    ins = [t.requires_grad_() for t in (xs, w_up, w_down)]
+    dys = rnd(60, 64, seed=103)
+    odd = torch.empty(60 * 64 + 1, dtype=BF, device="cuda")[1:].view(60, 64).copy_(dys)
+    want = torch.autograd.grad(experts.expert_ffn(*ins, offsets), ins, dys)
+    for g in (odd, dys.t().contiguous().t()):
+        got = torch.autograd.grad(experts.expert_ffn(*ins, offsets), ins, g)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    x = rnd(30, 64, seed=104).requires_grad_()
+    index = index_of(30, 2, 4, 105, 0.1)
+    a, = torch.autograd.grad(experts.expert_dispatch(x, index, 4)[0], x, dys)
+    b, = torch.autograd.grad(experts.expert_dispatch(x, index, 4)[0], x, odd)
+    assert torch.equal(a, b)
 
 
 def test_empty_inputs():
