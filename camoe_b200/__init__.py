@@ -6,8 +6,11 @@ Public entry points:
   camoe/backbone.py (``init_rwkv7_cuda``, ``RWKV7_ClampW``, ``RUN_CUDA_RWKV7``).
 * ``camoe_b200.ops`` — ``wkv7_forward`` / ``wkv7_backward`` on [B, T, H, 64]
   CUDA tensors (any T, head ranges, algorithm choice).
+* ``camoe_b200.timemix`` — the RWKV-7 time mix; ``camoe_b200.experts`` and
+  ``camoe_b200.adapters`` — the expert layer behind it and per-request low-rank
+  adapters; ``camoe_b200.block`` — a block of them.
 * ``camoe_b200.launcher`` — one-process-per-GPU batch/head sharding.
-* ``include/camoe_wkv7.h`` — the C ABI underneath, for non-Python callers.
+* ``include/camoe_*.h`` — the C ABI underneath, for non-Python callers.
 """
 from . import ops  # noqa: F401
 from ._lib import CamoeError  # noqa: F401
