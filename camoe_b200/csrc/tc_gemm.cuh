@@ -367,14 +367,21 @@ struct Tiles {
 };
 
 // A value as its bf16 rounding and 8 more bits: what an operand of the products
-// cannot hold but a derivative can use.
-__device__ __forceinline__ int low_bits(float v, bf16 hi) {
-  const int d = static_cast<int>(__float_as_uint(v) - (static_cast<uint32_t>(__bfloat16_as_ushort(hi)) << 16));
-  const int q = (d + 128) >> 8;
-  return q > 127 ? 127 : q;
+// cannot hold but a derivative can use.  d: the value's bits behind the rounded
+// one's, rounded to a multiple of 256; its second byte is kept.
+__device__ __forceinline__ int low_word(float v, uint32_t hi) {
+  const int d = static_cast<int>(__float_as_uint(v) - hi + 128u);
+  return d < 32767 ? d : 32767;
 }
-__device__ __forceinline__ float with_low(float hi, int low) {
-  return __uint_as_float(__float_as_uint(hi) + (static_cast<uint32_t>(low) << 8));
+__device__ __forceinline__ int low_bits(float v, bf16 hi) {
+  return low_word(v, static_cast<uint32_t>(__bfloat16_as_ushort(hi)) << 16) >> 8;
+}
+// byte i of `low`, signed, in place
+template <int i>
+__device__ __forceinline__ float with_low(uint32_t hi, uint32_t low) {
+  uint32_t d;  // bytes 3 and 2: the byte's sign (bit 3 of a selector), 1: the byte, 0: zero
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(low), "r"(0u), "n"((8 + i) << 12 | (8 + i) << 8 | i << 4 | 4));
+  return __uint_as_float(hi + d);
 }
 // one instruction, 1 ulp: its result is multiplied and rounded to bf16
 __device__ __forceinline__ float fast_sqrt(float x) {
@@ -382,9 +389,17 @@ __device__ __forceinline__ float fast_sqrt(float x) {
   asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float relu(float x) {  // NaN stays NaN
+  float y;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+  return y;
+}
 template <int kEpi>
 __device__ __forceinline__ float finish(float x, float aux, float scale) {
-  if (kEpi == kRelu2) return x < 0.0f ? 0.0f : x * x;  // NaN stays NaN
+  if (kEpi == kRelu2) {
+    const float y = relu(x);
+    return y * y;
+  }
   if (kEpi == kDRelu2) return x * (2.0f * fast_sqrt(aux));
   if (kEpi == kScale) return x * scale;
   return x;
@@ -685,27 +700,33 @@ __global__ void __launch_bounds__(kThreads, 1)
             av = *reinterpret_cast<const uint4*>(out + out_at(lane, q));
             if (a.low != nullptr) lv = *reinterpret_cast<const uint2*>(lows + low_at(lane, q / 2) + 8 * (q % 2));
           }
-          const bf16* ah = reinterpret_cast<const bf16*>(&av);
-          const int8_t* al = reinterpret_cast<const int8_t*>(&lv);
-          uint4 o;
-          __nv_bfloat162* oh = reinterpret_cast<__nv_bfloat162*>(&o);
-          uint32_t l[2] = {0u, 0u};
+          const uint32_t ah[4] = {av.x, av.y, av.z, av.w}, al[2] = {lv.x, lv.y};
+          uint32_t o4[4], l[2] = {0u, 0u};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float h0 = 0.0f, h1 = 0.0f;
+          for (int e = 0; e < 2; ++e) {  // four columns
+            float y[4], h[4] = {};
             if (kEpi == kDRelu2) {
-              h0 = with_low(__bfloat162float(ah[2 * e]), al[2 * e]);
-              h1 = with_low(__bfloat162float(ah[2 * e + 1]), al[2 * e + 1]);
+              h[0] = with_low<0>(ah[2 * e] << 16, al[e]);
+              h[1] = with_low<1>(ah[2 * e] & 0xffff0000u, al[e]);
+              h[2] = with_low<2>(ah[2 * e + 1] << 16, al[e]);
+              h[3] = with_low<3>(ah[2 * e + 1] & 0xffff0000u, al[e]);
             }
-            const float y0 = finish<kEpi>(__uint_as_float(v[8 * q + 2 * e]), h0, scale);
-            const float y1 = finish<kEpi>(__uint_as_float(v[8 * q + 2 * e + 1]), h1, scale);
-            oh[e] = __floats2bfloat162_rn(y0, y1);
-            if (kEpi == kRelu2) {
-              const uint32_t both = (static_cast<uint32_t>(low_bits(y0, oh[e].x)) & 255u) |
-                                    (static_cast<uint32_t>(low_bits(y1, oh[e].y)) & 255u) << 8;
-              l[e / 2] |= both << (16 * (e % 2));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = finish<kEpi>(__uint_as_float(v[8 * q + 4 * e + i]), h[i], scale);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const __nv_bfloat162 two = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
+              o4[2 * e + i] = *reinterpret_cast<const uint32_t*>(&two);
+            }
+            if (kEpi == kRelu2 && a.low != nullptr) {
+              const uint32_t l01 = __byte_perm(low_word(y[0], o4[2 * e] << 16),
+                                               low_word(y[1], o4[2 * e] & 0xffff0000u), 0x0051);
+              const uint32_t l23 = __byte_perm(low_word(y[2], o4[2 * e + 1] << 16),
+                                               low_word(y[3], o4[2 * e + 1] & 0xffff0000u), 0x0051);
+              l[e] = __byte_perm(l01, l23, 0x5410);
             }
           }
+          const uint4 o = make_uint4(o4[0], o4[1], o4[2], o4[3]);
           *reinterpret_cast<uint4*>(out + out_at(lane, q)) = o;
           if (kEpi == kRelu2 && a.low != nullptr) {
             if (q % 2 == 0) {
