@@ -8,11 +8,11 @@
 //
 // Up to kSmallSlots slots one launch does it all: each token's block counts its
 // own slots' rows by reading the whole index once (a warp per slot) and copies
-// its row.  Above that the slots are counted per chunk, every chunk's block places
-// its own slots (adding up the counts of the chunks before it, and a warp's of the
-// warps before it), and the copy follows; the launches overlap (programmatic
-// dependent launches), so that the index and x are loaded by the time the counts
-// and the rows are known.
+// its row.  Above that every chunk of slots has a block that places them: it adds
+// up the slots of the chunks before it (up to 8192 slots by reading the whole index
+// itself, above from counts per chunk that a first launch makes) and a warp's of
+// the warps before it.  The copy follows; the launches overlap (programmatic
+// dependent launches), so that x is loaded by the time the rows are known.
 //
 // The copies are bound by HBM: a thread holds 16 bytes (or one element where the
 // width or an address is no multiple of 16 bytes) of a row of each of kTokens
@@ -169,6 +169,9 @@ inline int64_t chunk_of(int64_t S) {
   const int64_t c = ((S + 255) / 256 + kSortThreads - 1) / kSortThreads * kSortThreads;
   return c > 2 * kSortThreads ? c : 2 * kSortThreads;
 }
+// Whether each block counts all slots itself: one launch less (6 us for 7001 slots, 6.5
+// in two launches; 16384 slots 10.7 and 6.5), where its counters fit.
+inline bool alone(int64_t S, int64_t E) { return S <= 8192 && E < 512; }
 inline int64_t chunks_of(int64_t S) { return (S + chunk_of(S) - 1) / chunk_of(S); }
 
 // slots of each expert in each chunk: counts[chunk][expert]
@@ -215,13 +218,44 @@ __global__ void __launch_bounds__(kSortThreads)
     for (int u = 0; u < kSortDeep; ++u)
       if (bin[u] <= E) atomicAdd(&mine[bin[u]], 1);
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the counts
-  const int chunks = gridDim.x;
-  for (int i = threadIdx.x; i < chunks * (E + 1); i += kSortThreads) {
-    const int n = counts[i], c = i / (E + 1), e = i - c * (E + 1);
-    if (n == 0) continue;
-    atomicAdd(&all[e], n);
-    if (c < static_cast<int>(blockIdx.x)) atomicAdd(&first[e], n);
+  if (counts == nullptr) {  // the block counts all slots for itself, a warp's in its own counters
+    int* temp = first + E + 1;  // [kSortWarps][E + 1]
+    int* own = temp + warp * (E + 1);
+    for (int i = threadIdx.x; i < kSortWarps * (E + 1); i += kSortThreads) temp[i] = 0;
+    __syncthreads();
+    const int64_t cut = blockIdx.x * chunk;
+    for (int half = 0; half < 2; ++half) {  // the slots before the chunk, then the others
+      const int64_t end = half == 0 ? cut : S;
+      for (int64_t t = (half == 0 ? 0 : cut) + warp * 32; t < end; t += 32 * kSortWarps * kSortDeep) {
+        int bin[kSortDeep];
+#pragma unroll
+        for (int u = 0; u < kSortDeep; ++u) {
+          const int64_t s = t + u * 32 * kSortWarps + lane;
+          bin[u] = s < end ? bin_of(index, s, E) : E + 1;
+        }
+#pragma unroll
+        for (int u = 0; u < kSortDeep; ++u) {
+          const unsigned same = __match_any_sync(kFull, bin[u]);
+          if (bin[u] <= E && (same & ((1u << lane) - 1u)) == 0) own[bin[u]] += __popc(same);
+          __syncwarp();
+        }
+      }
+      __syncthreads();
+      for (int e = threadIdx.x; e <= E; e += kSortThreads) {
+        int n = 0;
+        for (int w = 0; w < kSortWarps; ++w) n += temp[w * (E + 1) + e];
+        (half == 0 ? first : all)[e] = n;
+      }
+    }
+  } else {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the counts
+    const int chunks = gridDim.x;
+    for (int i = threadIdx.x; i < chunks * (E + 1); i += kSortThreads) {
+      const int n = counts[i], c = i / (E + 1), e = i - c * (E + 1);
+      if (n == 0) continue;
+      atomicAdd(&all[e], n);
+      if (c < static_cast<int>(blockIdx.x)) atomicAdd(&first[e], n);
+    }
   }
   __syncthreads();
   // rows before expert e: a scan over the experts, `per` of them per thread
@@ -482,9 +516,12 @@ int sort(const P* x, const I* index, P* xs, int* offsets, int* position, int* so
   }
   const int64_t chunk = chunk_of(S);
   const unsigned g = static_cast<unsigned>(chunks_of(S));
-  count_kernel<I><<<g, kSortThreads, 0, st>>>(index, work, S, chunk, E);
-  if (const int e = camoe::tm::status(cudaGetLastError())) return e;
-  const int smem = (kSortWarps + 2) * (E + 1) * static_cast<int>(sizeof(int));
+  const bool solo = alone(S, E);
+  if (!solo) {
+    count_kernel<I><<<g, kSortThreads, 0, st>>>(index, work, S, chunk, E);
+    if (const int e = camoe::tm::status(cudaGetLastError())) return e;
+  }
+  const int smem = ((solo ? 2 : 1) * kSortWarps + 2) * (E + 1) * static_cast<int>(sizeof(int));
   const auto place = place_kernel<I, kKeep>;
   if (smem > 48 * 1024)
     if (const int e = camoe::tm::status(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))
@@ -498,8 +535,9 @@ int sort(const P* x, const I* index, P* xs, int* offsets, int* position, int* so
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (const int e = camoe::tm::status(cudaLaunchKernelEx(&cfg, place, index, static_cast<const int*>(work), offsets,
+  cfg.numAttrs = solo ? 0 : 1;  // by itself it reads the index at once
+  if (const int e = camoe::tm::status(cudaLaunchKernelEx(&cfg, place, index,
+                                                         static_cast<const int*>(solo ? nullptr : work), offsets,
                                                          position, source, S, chunk, E)))
     return e;
   if (xs == nullptr || V == 0) return 0;
@@ -507,6 +545,7 @@ int sort(const P* x, const I* index, P* xs, int* offsets, int* position, int* so
   cfg.gridDim = dim3(static_cast<unsigned>(blocks(N, b, kTokens) + (kKeep ? 0 : kTailBlocks)));
   cfg.blockDim = b;
   cfg.dynamicSmemBytes = 0;
+  cfg.numAttrs = 1;
   return camoe::tm::status(cudaLaunchKernelEx(&cfg, copy_kernel<P>, x, static_cast<const int*>(position),
                                               static_cast<const int*>(offsets), xs, N, k, E, V, !kKeep));
 }
@@ -524,7 +563,7 @@ int sort_index(const void* x, const void* index, int index_bytes, void* xs, int*
 }
 
 size_t sort_bytes(int64_t N, int64_t k, int64_t E) {
-  if (N * k <= kSmallSlots) return 0;
+  if (N * k <= kSmallSlots || alone(N * k, E)) return 0;
   return static_cast<size_t>(chunks_of(N * k)) * static_cast<size_t>(E + 1) * sizeof(int);
 }
 

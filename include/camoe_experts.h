@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-/* Bytes of workspace of camoe_ex_dispatch (0 for up to 2048 slots: work may be NULL). */
+/* Bytes of workspace of camoe_ex_dispatch (may be 0, then work may be NULL). */
 size_t camoe_ex_dispatch_work_bytes(int64_t N, int64_t k, int64_t E);
 
 /* Sort the slots and copy the tokens: index [N, k] holds the chosen experts

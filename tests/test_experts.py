@@ -37,10 +37,10 @@ def test_dispatch_statuses():
     for bad in (dict(N=-1), dict(k=0), dict(E=0), dict(C=-1), dict(index=None), dict(offsets=None), dict(x=None)):
         assert dispatch(**bad) == _lib.ERR_INVALID_ARG, bad
     assert dispatch(N=1 << 31) == _lib.ERR_SHAPE
-    need = _lib.lib().camoe_ex_dispatch_work_bytes(5000, 2, 8)
+    need = _lib.lib().camoe_ex_dispatch_work_bytes(50000, 2, 8)
     assert need > 0 and _lib.lib().camoe_ex_dispatch_work_bytes(4, 2, 8) == 0
-    assert dispatch(N=5000, nbytes=need - 1) == _lib.ERR_WORKSPACE
-    assert dispatch(N=5000, work=None) == _lib.ERR_INVALID_ARG
+    assert dispatch(N=50000, nbytes=need - 1) == _lib.ERR_WORKSPACE
+    assert dispatch(N=50000, work=None) == _lib.ERR_INVALID_ARG
     assert _lib.lib().camoe_ex_dispatch_work_bytes(-1, 2, 8) == 0
 
 

@@ -49,11 +49,15 @@ def close(got, want, tol, name):
 def plain_sort(index, E):
     """(offsets, position, source) by definition, on the host."""
     flat = index.cpu().reshape(-1).tolist()
-    order = [s for e in range(E) for s in range(len(flat)) if flat[s] == e]
+    of = [[] for _ in range(E)]
+    for s, e in enumerate(flat):
+        if 0 <= e < E:
+            of[e].append(s)
+    order = [s for slots in of for s in slots]
     position, source = [-1] * len(flat), order + [-1] * (len(flat) - len(order))
     for p, s in enumerate(order):
         position[s] = p
-    offsets = [sum(0 <= e < b for e in flat) for b in range(E + 1)]
+    offsets = [sum(len(slots) for slots in of[:b]) for b in range(E + 1)]
     return offsets, position, source
 
 
@@ -65,7 +69,7 @@ def index_of(N, k, E, seed, empty=0.0, dtype=torch.int64):
 
 SORTS = [  # N, k, E: one slot, the one-launch path's ends, chunk borders, many experts
     (1, 1, 1), (1, 2, 8), (7, 3, 5), (1024, 2, 8), (1025, 2, 8), (683, 3, 1024), (2048, 1, 3), (5000, 2, 61),
-    (4096, 4, 200),
+    (4096, 4, 200), (8192, 4, 8), (32769, 1, 7),
 ]
 
 
