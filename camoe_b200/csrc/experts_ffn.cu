@@ -1,5 +1,6 @@
 // The experts' squared-ReLU products over sorted rows (declared in
-// include/camoe_experts.h): forward in two grouped products, backward in four.
+// include/camoe_experts.h): forward in two grouped products, backward in four
+// (three launches).
 //
 //   h    = relu(xs w_up^T)^2          rows, K = C, k contiguous in both
 //   ys   = h w_down^T                 rows, K = F
@@ -149,19 +150,20 @@ int camoe_ex_ffn_bwd(const void* dys, const void* xs, const void* w_up, const vo
     a.zero_tail = 1;
     if (const int st = rows_product<true, tc::kPlain>(dpre, w_up, a, E, s)) return st;
   }
-  if (dw_up != nullptr) {
-    if (xs == nullptr) return 1;
-    tc::Args a = args(offsets, E, R, C, 0, dw_up);
-    a.M = static_cast<int>(F);
-    if (const int st = tc::launch<2, 256, true, true, tc::kWeights, tc::kPlain>({dpre, F, R, 1}, {xs, C, R, 1}, {}, {}, a, s))
-      return st;
-  }
+  if (dw_up == nullptr && dw_down == nullptr) return 0;
+  if (dw_up != nullptr && xs == nullptr) return 1;
+  // both weight gradients in one launch: one start and end, one last round of tiles
+  const tc::Matrix up[2] = {{dpre, F, R, 1}, {xs, C, R, 1}}, down[2] = {{dys, C, R, 1}, {h, F, R, 1}};
+  tc::Args a = args(offsets, E, R, dw_up != nullptr ? C : F, 0, dw_up != nullptr ? dw_up : dw_down);
+  a.M = static_cast<int>(dw_up != nullptr ? F : C);
+  if (dw_up == nullptr)
+    return tc::launch<2, 256, true, true, tc::kWeights, tc::kPlain>(down[0], down[1], {}, {}, a, s);
   if (dw_down != nullptr) {
-    tc::Args a = args(offsets, E, R, F, 0, dw_down);
-    a.M = static_cast<int>(C);
-    return tc::launch<2, 256, true, true, tc::kWeights, tc::kPlain>({dys, C, R, 1}, {h, F, R, 1}, {}, {}, a, s);
+    a.M2 = static_cast<int>(C);
+    a.N2 = static_cast<int>(F);
+    a.out2 = static_cast<bf16*>(dw_down);
   }
-  return 0;
+  return tc::launch<2, 256, true, true, tc::kWeights, tc::kPlain>(up[0], up[1], down[0], down[1], a, s);
 }
 
 }  // extern "C"

@@ -68,6 +68,8 @@ struct Args {
   int64_t R;             // rows of A (the sorted arrays)
   int M, N, K;           // M: weight gradients only
   int K2;                // kJoined: depth of the blocks (maps ma2: blocks, mb2: B2)
+  int M2, N2;            // kWeights: a second product in the same launch, or 0 (maps ma2, mb2, mlow: out2)
+  bf16* out2;
   int zero_tail;         // write zeros to the rows behind the last group
   bf16* out;
   int8_t* low;           // [R, low_stride(N)] (kRelu2, kDRelu2) or null: the 8 bits of the value below bf16's
@@ -287,18 +289,21 @@ struct Tile {
   int nk1, nk;         // pieces of the first pair, of both
   int tile;            // kBlocks: block; kJoined: row tile
   int64_t lead;        // kBlocks: rows of the tile before the group's
+  bool second;         // kWeights: of the second product
 };
 
 template <int kCG, int kBN, int kMode>
 struct Tiles {
   const Args& a;
   const Control& c;
-  int nt, mt;
+  int nt, mt, nt2, mt2;
   int whole, jobs;  // tiles done whole, and these with the halves of the others
   __device__ Tiles(const Args& args, const Control& ctl) : a(args), c(ctl) {
     nt = (a.N + kBN - 1) / kBN;
     mt = kMode == kWeights ? (a.M + (128 * kCG) - 1) / (128 * kCG) : 0;
-    const int total = kMode == kWeights ? a.groups * mt * nt
+    nt2 = kMode == kWeights ? (a.N2 + kBN - 1) / kBN : 0;
+    mt2 = kMode == kWeights ? (a.M2 + (128 * kCG) - 1) / (128 * kCG) : 0;
+    const int total = kMode == kWeights ? a.groups * (mt * nt + mt2 * nt2)
                       : kMode == kJoined ? static_cast<int>((a.R + 128 * kCG - 1) / (128 * kCG)) * nt
                                          : c.tiles[a.groups] * nt;
     // Tiles left for a last round that would leave half of the workers or more
@@ -325,13 +330,16 @@ struct Tiles {
   }
   __device__ Tile get(int job) const {
     Tile x;
-    const int t = job < whole ? job : whole + (job - whole) / 2;
-    const int rt = t / nt;
+    int t = job < whole ? job : whole + (job - whole) / 2;
+    x.second = kMode == kWeights && t >= a.groups * mt * nt;
+    if (x.second) t -= a.groups * mt * nt;
+    const int nts = x.second ? nt2 : nt, mts = x.second ? mt2 : mt;
+    const int rt = t / nts;
     x.width = job < whole ? kBN : kBN / 2;
-    x.n0 = (t - rt * nt) * kBN + (job < whole ? 0 : (job - whole) % 2 * (kBN / 2));
+    x.n0 = (t - rt * nts) * kBN + (job < whole ? 0 : (job - whole) % 2 * (kBN / 2));
     if (kMode == kWeights) {
-      x.group = rt / mt;
-      x.m0 = (rt - x.group * mt) * (128 * kCG);
+      x.group = rt / mts;
+      x.m0 = (rt - x.group * mts) * (128 * kCG);
       x.row0 = first(x.group);
       x.row1 = first(x.group + 1);
       x.nk1 = x.nk = x.row1 > x.row0 ? static_cast<int>((x.row1 - x.row0 + kBK - 1) / kBK) : 0;
@@ -527,10 +535,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t sa = ring0 + s * kStage, sb = sa + Sh::kABytes;
           if (kMode == kWeights) {
             const int r = static_cast<int>(x.row0) + j * kBK;
-            load_box<kCG>(sa, &ma, m, r, 0, bar);
-            load_box<kCG>(sa + kBox, &ma, m + 64, r, 0, bar);
-            load_box<kCG>(sb, &mb, n, r, 0, bar);
-            for (int q = 1; q < boxes; ++q) load_box<kCG>(sb + q * kBox, &mb, n + 64 * q, r, 0, bar);
+            const CUtensorMap* pa = x.second ? &ma2 : &ma;
+            const CUtensorMap* pb = x.second ? &mb2 : &mb;
+            load_box<kCG>(sa, pa, m, r, 0, bar);
+            load_box<kCG>(sa + kBox, pa, m + 64, r, 0, bar);
+            load_box<kCG>(sb, pb, n, r, 0, bar);
+            for (int q = 1; q < boxes; ++q) load_box<kCG>(sb + q * kBox, pb, n + 64 * q, r, 0, bar);
           } else {
             const bool one = kMode != kJoined || j < x.nk1;
             const int k = one ? j * kBK : part * kBK;
@@ -636,12 +646,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Tile x = tiles.get(t);
       const int b = done & 1;
       const bool have = x.nk > 0;
+      const int M = x.second ? a.M2 : a.M, N = x.second ? a.N2 : a.N;
+      bf16* const dest = x.second ? a.out2 : a.out;
       // the warp's 32 rows: the first, and how many of them exist
       const int in_tile = static_cast<int>(rank) * 128 + 32 * quarter;
-      const int64_t row0 = (kMode == kWeights  ? static_cast<int64_t>(x.group) * a.M + x.m0
+      const int64_t row0 = (kMode == kWeights  ? static_cast<int64_t>(x.group) * M + x.m0
                             : kMode == kBlocks ? static_cast<int64_t>(x.tile) * Sh::kBM
                                                : x.row0) + in_tile;
-      const int64_t left = (kMode == kWeights ? a.M - x.m0 : kMode == kBlocks ? Sh::kBM : x.row1 - x.row0) - in_tile;
+      const int64_t left = (kMode == kWeights ? M - x.m0 : kMode == kBlocks ? Sh::kBM : x.row1 - x.row0) - in_tile;
       // kBlocks: this lane's row is the group's
       const bool live = kMode != kBlocks || (in_tile + lane >= x.lead && x.row0 + in_tile + lane < x.row1);
       const int rows = left < 32 ? (left > 0 ? static_cast<int>(left) : 0) : 32;
@@ -649,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int to = 0;  // where this lane's row goes
       if (kMode != kWeights && a.scatter != nullptr && lane < rows) to = a.scatter[row0 + lane];
       const int begin = half * (x.width / 2), end = begin + x.width / 2;
-      const int cols = a.N - x.n0 < end ? a.N - x.n0 : end;
+      const int cols = N - x.n0 < end ? N - x.n0 : end;
       if (kEpi == kDRelu2 && rows > 0 && begin < cols) {
         if (lane == 0) bulk_wait_read();
         fetch(steps, x.n0 + begin, row0);
@@ -745,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
-            store_box(&mo, sm_addr(out), n, static_cast<int>(row0));
+            store_box(x.second ? &mlow : &mo, sm_addr(out), n, static_cast<int>(row0));
             if (kEpi == kRelu2 && a.low != nullptr) store_box(&mlow, sm_addr(lows), n, static_cast<int>(row0));
             bulk_commit();
           }
@@ -757,16 +769,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 4; ++i) {
           const int r = 8 * i + (lane >> 2), m = n + 8 * (lane & 3);
           const int64_t dst = kMode != kWeights && a.scatter != nullptr ? __shfl_sync(0xffffffffu, to, r) : row0 + r;
-          if (r < rows && m < a.N)
-            *reinterpret_cast<uint4*>(a.out + dst * a.N + m) =
+          if (r < rows && m < N)
+            *reinterpret_cast<uint4*>(dest + dst * N + m) =
                 *reinterpret_cast<const uint4*>(out + out_at(r, lane & 3));
         }
         if (kEpi == kRelu2 && a.low != nullptr) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int r = 16 * i + (lane >> 1), m = n + 16 * (lane & 1);
-            if (r >= rows || m >= a.N) continue;
-            *reinterpret_cast<uint4*>(a.low + (row0 + r) * low_stride(a.N) + m) =
+            if (r >= rows || m >= N) continue;
+            *reinterpret_cast<uint4*>(a.low + (row0 + r) * low_stride(N) + m) =
                 *reinterpret_cast<const uint4*>(lows + low_at(r, lane & 1));
           }
         }

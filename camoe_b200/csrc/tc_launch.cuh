@@ -58,7 +58,7 @@ int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2,
   m[2] = m[4] = m[5] = m[0], m[3] = m[1];  // where a kernel has no use for them
   if (kEpi == kDRelu2)  // A2: h
     ok = ok && tma::encode_2d_rows(&m[2], A2.base, 2 * A2.inner, A2.rows, 64, 32);
-  else if (kMode == kJoined)
+  else if (kMode == kJoined || (kMode == kWeights && a.M2 > 0))
     ok = ok && tma::encode_3d_sw128(&m[2], A2.base, A2.inner, A2.rows, A2.depth, ra) &&
          tma::encode_3d_sw128(&m[3], B2.base, B2.inner, B2.rows, B2.depth, rb);
   // the epilogue's boxes of 32 x 32
@@ -67,6 +67,8 @@ int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2,
                                    kMode == kWeights  ? static_cast<int64_t>(a.groups) * a.M
                                    : kMode == kBlocks ? most_blocks(a.R, a.groups, Sh::kBM) * Sh::kBM
                                                       : a.R, 64, 32);
+  if (kMode == kWeights && a.M2 > 0)
+    ok = ok && tma::encode_2d_rows(&m[5], a.out2, 2 * static_cast<int64_t>(a.N2), static_cast<int64_t>(a.groups) * a.M2, 64, 32);
   if (a.low != nullptr) ok = ok && tma::encode_2d_rows(&m[5], a.low, low_stride(a.N), a.R, 32, 32);
   if (!ok) return camoe::tm::status(cudaErrorInvalidValue);
   const int64_t nt = (a.N + kBN - 1) / kBN;
@@ -74,10 +76,14 @@ int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2,
                      : kMode == kJoined ? (a.R + Sh::kBM - 1) / Sh::kBM
                      : kMode == kBlocks ? most_blocks(a.R, a.groups, Sh::kBM)
                                         : a.R / Sh::kBM + (a.R < a.groups ? a.R : a.groups);
-  if (nt * rt > 0x7fffffffLL) return 3;  // CAMOE_ERR_SHAPE
+  const int64_t more = kMode == kWeights ? static_cast<int64_t>(a.groups) * ((a.M2 + Sh::kBM - 1) / Sh::kBM) *
+                                               ((a.N2 + kBN - 1) / kBN)
+                                         : 0;
+  const int64_t tiles = nt * rt + more;
+  if (tiles > 0x3fffffffLL) return 3;  // CAMOE_ERR_SHAPE
   int64_t pairs = sm_count() / kCG;
   if (pairs < 1) return camoe::tm::status(cudaErrorNoDevice);
-  if (2 * nt * rt < pairs) pairs = nt * rt > 0 ? 2 * nt * rt : 1;  // a tile may be done as two halves
+  if (2 * tiles < pairs) pairs = tiles > 0 ? 2 * tiles : 1;  // a tile may be done as two halves
   const auto kernel = gemm_kernel<kCG, kBN, kAMN, kBMN, kMode, kEpi>;
   static std::atomic<uint64_t> opted{0};
   constexpr int smem = smem_bytes<kCG, kBN, kEpi>();
