@@ -129,7 +129,7 @@ int check(int64_t N, int64_t C, int64_t M, int64_t D, int64_t L) {
 
 template <int kBN>
 int low_product(const bf16* xs, const void* down, const tc::Args& a, int64_t L, cudaStream_t st) {
-  return tc::launch<2, kBN, false, false, tc::kBlocks, tc::kScale>({xs, a.K, a.R, 1}, {down, a.K, a.N, L}, {}, {}, a, st);
+  return tc::launch<kBN, false, false, tc::kBlocks, tc::kScale>({xs, a.K, a.R, 1}, {down, a.K, a.N, L}, {}, {}, a, st);
 }
 
 }  // namespace adapt
@@ -210,7 +210,7 @@ int camoe_ad_linear(const void* x, const void* weight, const void* down, const v
   a.out = static_cast<bf16*>(y);
   a.scale = nullptr;
   a.scatter = source;
-  return tc::launch<2, 256, false, false, tc::kJoined, tc::kPlain>(
+  return tc::launch<256, false, false, tc::kJoined, tc::kPlain>(
       {xs, C, N, 1}, {weight, C, M, 1}, {low, D, blocks(N, L) * kTile, 1}, {up, D, M, L}, a, s);
 }
 

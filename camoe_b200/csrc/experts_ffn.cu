@@ -12,8 +12,8 @@
 // h and dpre are held in bf16, the type of the products' operands.  relu(pre) is
 // not kept: it is sqrt(h).  For the backward h is kept with 8 bits more than
 // bf16 (one byte each): without them the root of the rounded h would add half of
-// its rounding error to dpre's own (2.5e-3 against 2.4e-3 of dxs and dw_up in the
-// 2-norm, where one rounding is 1.7e-3).
+// its rounding error to dpre's own (2.49e-3 against 2.35e-3 of dxs and dw_up in the
+// 2-norm, 16384 rows x 1024 x 4096, where one rounding is 1.7e-3).
 #include "camoe_experts.h"
 #include "tc_gemm.cuh"
 #include "tc_launch.cuh"
@@ -74,7 +74,7 @@ tc::Args args(const int* offsets, int64_t E, int64_t R, int64_t N, int64_t K, vo
 template <bool kBMN, int kEpi>
 int rows_product(const void* x, const void* w, const tc::Args& a, int64_t E, cudaStream_t st,
                  const void* h = nullptr) {
-  return tc::launch<2, 256, false, kBMN, tc::kRows, kEpi>(
+  return tc::launch<256, false, kBMN, tc::kRows, kEpi>(
       {x, a.K, a.R, 1}, kBMN ? tc::Matrix{w, a.N, a.K, E} : tc::Matrix{w, a.K, a.N, E}, {h, a.N, a.R, 1},
       {}, a, st);
 }
@@ -157,13 +157,13 @@ int camoe_ex_ffn_bwd(const void* dys, const void* xs, const void* w_up, const vo
   tc::Args a = args(offsets, E, R, dw_up != nullptr ? C : F, 0, dw_up != nullptr ? dw_up : dw_down);
   a.M = static_cast<int>(dw_up != nullptr ? F : C);
   if (dw_up == nullptr)
-    return tc::launch<2, 256, true, true, tc::kWeights, tc::kPlain>(down[0], down[1], {}, {}, a, s);
+    return tc::launch<256, true, true, tc::kWeights, tc::kPlain>(down[0], down[1], {}, {}, a, s);
   if (dw_down != nullptr) {
     a.M2 = static_cast<int>(C);
     a.N2 = static_cast<int>(F);
     a.out2 = static_cast<bf16*>(dw_down);
   }
-  return tc::launch<2, 256, true, true, tc::kWeights, tc::kPlain>(up[0], up[1], down[0], down[1], a, s);
+  return tc::launch<256, true, true, tc::kWeights, tc::kPlain>(up[0], up[1], down[0], down[1], a, s);
 }
 
 }  // extern "C"

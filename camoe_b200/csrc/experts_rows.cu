@@ -169,8 +169,8 @@ inline int64_t chunk_of(int64_t S) {
   const int64_t c = ((S + 255) / 256 + kSortThreads - 1) / kSortThreads * kSortThreads;
   return c > 2 * kSortThreads ? c : 2 * kSortThreads;
 }
-// Whether each block counts all slots itself: one launch less (6 us for 7001 slots, 6.5
-// in two launches; 16384 slots 10.7 and 6.5), where its counters fit.
+// Whether each block counts all slots itself, one launch less, where its counters fit.
+// Kernel times: 7001 slots 6.0 us, 3.3 + 4.6 in two launches; 16384 slots 10.7 us, 3.1 + 4.3.
 inline bool alone(int64_t S, int64_t E) { return S <= 8192 && E < 512; }
 inline int64_t chunks_of(int64_t S) { return (S + chunk_of(S) - 1) / chunk_of(S); }
 

@@ -15,7 +15,7 @@
 //     p's tile of sum over d of block[p][d] B2_g[n][d]: a group's product reaches
 //     its own rows only, as more of the same sum.
 //
-// One CTA (or a pair of CTAs on two SMs, kCG = 2) per tile of 128 kCG rows x kBN
+// One pair of CTAs on two SMs (kCG = 2) per tile of 128 kCG rows x kBN
 // columns, persistent over the tiles:
 //   * warp 0 streams 64-deep pieces of A and B through a ring of stages by TMA
 //     (128-byte swizzle); a piece that passes the end of a matrix reads zeros;
@@ -44,6 +44,7 @@
 namespace camoe {
 namespace tc {
 
+constexpr int kCG = 2;            // CTAs of a tile: a pair, on two SMs
 constexpr int kBK = 64;           // depth of a stage: one 128-byte swizzled row of bf16
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;  // producer, product issue, epilogue
@@ -80,7 +81,7 @@ struct Args {
 // Per epilogue warp: 32 rows x 32 columns of bf16, and of bytes
 constexpr uint32_t kOutBytes = 32 * 64, kLowBytes = 32 * 32;
 
-template <int kCG, int kBN, int kEpi>
+template <int kBN, int kEpi>
 struct Shape {
   static constexpr int kBM = 128 * kCG;
   static constexpr uint32_t kABytes = 128 * 128;          // per CTA and stage
@@ -102,20 +103,19 @@ struct Control {
   int first[kMaxGroups + 1];  // the groups' first rows, clamped to R
 };
 
-template <int kCG, int kBN, int kEpi>
+template <int kBN, int kEpi>
 __host__ __device__ constexpr int smem_bytes() {
-  using Sh = Shape<kCG, kBN, kEpi>;
+  using Sh = Shape<kBN, kEpi>;
   return Sh::kStages * static_cast<int>(Sh::kABytes + Sh::kBBytes) + static_cast<int>(Sh::kStaging) +
          static_cast<int>(sizeof(Control)) + 1024;
 }
 
 // ---- PTX
 
-// mbarrier address in the CTA `rank` of the cluster (itself for a CTA alone)
-template <int kCG>
+// mbarrier address in the CTA `rank` of the pair
 __device__ __forceinline__ uint32_t bar_at(uint64_t* bar, uint32_t rank) {
   uint32_t a = sm_addr(bar);
-  if (kCG > 1) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(rank));
   return a;
 }
 // The scopes matter for speed: a release or an acquire at cluster scope waits
@@ -155,10 +155,10 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
 // box at (x, y, z) into this CTA's shared memory, completing on the barrier at `bar`
-template <int kCG>
+template <int kCtas>
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
                                          uint32_t bar) {
-  if (kCG > 1)
+  if (kCtas > 1)
     asm volatile(
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
         " [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
@@ -171,9 +171,9 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
-template <int kCG>
+template <int kCtas>
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
-  if (kCG > 1) {
+  if (kCtas > 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm_addr(slot)),
                  "r"(cols)
                  : "memory");
@@ -185,16 +185,16 @@ __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
 }
-template <int kCG>
+template <int kCtas>
 __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
-  if (kCG > 1)
+  if (kCtas > 1)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
   else
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
-template <int kCG>
+template <int kCtas>
 __device__ __forceinline__ void mma(uint32_t tmem, uint64_t da, uint64_t db, uint32_t idesc, bool add) {
-  if (kCG > 1)
+  if (kCtas > 1)
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem),
@@ -208,9 +208,9 @@ __device__ __forceinline__ void mma(uint32_t tmem, uint64_t da, uint64_t db, uin
         : "memory");
 }
 // arrive on the barrier (in both CTAs of a pair) once the products issued so far are done
-template <int kCG>
+template <int kCtas>
 __device__ __forceinline__ void commit(uint64_t* bar) {
-  if (kCG > 1)
+  if (kCtas > 1)
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
             sm_addr(bar)),
@@ -236,12 +236,8 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t src, 
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-template <int kCG>
 __device__ __forceinline__ void pair_sync() {
-  if (kCG > 1)
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  else
-    __syncthreads();
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // 32 consecutive accumulator columns of this thread's TMEM lane (the wait is in the
 // same statement, so that no use of v can be moved before it)
@@ -292,7 +288,7 @@ struct Tile {
   bool second;         // kWeights: of the second product
 };
 
-template <int kCG, int kBN, int kMode>
+template <int kBN, int kMode>
 struct Tiles {
   const Args& a;
   const Control& c;
@@ -419,12 +415,12 @@ __device__ __forceinline__ float finish(float x, float aux, float scale) {
 __device__ __forceinline__ uint32_t out_at(int r, int q) { return r * 64 + ((q ^ ((r >> 1) & 3)) << 4); }
 __device__ __forceinline__ uint32_t low_at(int r, int q) { return r * 32 + ((q ^ ((r >> 2) & 1)) << 4); }
 
-template <int kCG, int kBN, bool kAMN, bool kBMN, int kMode, int kEpi>
+template <int kBN, bool kAMN, bool kBMN, int kMode, int kEpi>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
                 const __grid_constant__ CUtensorMap ma2, const __grid_constant__ CUtensorMap mb2,
                 const __grid_constant__ CUtensorMap mo, const __grid_constant__ CUtensorMap mlow, const Args a) {
-  using Sh = Shape<kCG, kBN, kEpi>;
+  using Sh = Shape<kBN, kEpi>;
   constexpr int S = Sh::kStages, kBBox = Sh::box(kBMN);
   constexpr uint32_t kStage = Sh::kABytes + Sh::kBBytes;
   extern __shared__ __align__(128) unsigned char raw[];
@@ -432,8 +428,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char* staging = ring + S * kStage;
   Control& c = *reinterpret_cast<Control*>(staging + Sh::kStaging);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  uint32_t rank = 0;
-  if (kCG > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   const int worker = blockIdx.x / kCG, workers = gridDim.x / kCG;
 
   if (tid == 0) {
@@ -492,10 +488,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   fence_before();
   __syncthreads();
-  if (kCG > 1) pair_sync<kCG>();
+  pair_sync();
   fence_after();
   const uint32_t tmem = c.tmem, ring0 = sm_addr(ring);
-  const Tiles<kCG, kBN, kMode> tiles(a, c);
+  const Tiles<kBN, kMode> tiles(a, c);
 
   // Producer and product issue run as whole warps of which an elected lane acts: with
   // the operands uniform over the warp the issue is short (a branch on the lane
@@ -527,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (elect_one()) {
           const bool last = cut && j == x.nk - 1;
           // a piece to be cleared lands on this CTA's own barrier
-          const uint32_t bar = last ? sm_addr(&c.tail[s]) : bar_at<kCG>(&c.full[s], 0);
+          const uint32_t bar = last ? sm_addr(&c.tail[s]) : bar_at(&c.full[s], 0);
           if (last)
             mbar_arrive_expect_tx(&c.tail[s], bytes);
           else if (rank == 0)  // for both CTAs: the pair's loads complete on the leader's barrier
@@ -593,11 +589,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               *reinterpret_cast<uint4*>(ring + s * kStage + q * kBox + o) = make_uint4(0u, 0u, 0u, 0u);
           fence_proxy_async();
           __syncwarp();
-          if (kCG > 1 && rank != 0) {
-            if (lane == 0) arrive_release(bar_at<kCG>(&c.peer_tail[s], 0));
+          if (rank != 0) {
+            if (lane == 0) arrive_release(bar_at(&c.peer_tail[s], 0));
           } else {
-            if (kCG > 1 &&
-                !(ok = __all_sync(0xffffffffu, wait_acquire(&c.peer_tail[s], ((tail_phase >> s) & 1u) ^ 1u))))
+            if (!(ok = __all_sync(0xffffffffu, wait_acquire(&c.peer_tail[s], ((tail_phase >> s) & 1u) ^ 1u))))
               break;
             if (lane == 0) mbar_arrive(&c.full[s]);  // the stage's phase, which no load completes
             __syncwarp();
@@ -668,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (have && !(ok = warp_wait(&c.acc_full[b], static_cast<uint32_t>((done / 2) & 1)))) break;
       fence_after();
-      if (have && begin >= cols && lane == 0) arrive_at(bar_at<kCG>(&c.acc_empty[b], 0));
+      if (have && begin >= cols && lane == 0) arrive_at(bar_at(&c.acc_empty[b], 0));
 #pragma unroll 1
       for (int c0 = begin; c0 < cols; c0 += 32) {
         uint32_t v[32];
@@ -677,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (c0 + 32 >= cols) {  // read to the end: the accumulator is free
             fence_before();
             __syncwarp();
-            if (lane == 0) arrive_at(bar_at<kCG>(&c.acc_empty[b], 0));
+            if (lane == 0) arrive_at(bar_at(&c.acc_empty[b], 0));
           }
         } else {
 #pragma unroll
@@ -802,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   fence_before();
   __syncthreads();
-  if (kCG > 1) pair_sync<kCG>();
+  pair_sync();
   if (warp == 1) tmem_free<kCG>(tmem, Sh::kCols);
 }
 

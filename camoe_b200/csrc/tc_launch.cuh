@@ -47,9 +47,9 @@ cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
 
 // A, B and (kJoined) the second pair.  The box of an operand whose k is contiguous
 // has all its rows of a stage; one whose m or n is contiguous, 64 rows of k.
-template <int kCG, int kBN, bool kAMN, bool kBMN, int kMode, int kEpi>
+template <int kBN, bool kAMN, bool kBMN, int kMode, int kEpi>
 int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2, const Args& a, cudaStream_t s) {
-  using Sh = Shape<kCG, kBN, kEpi>;
+  using Sh = Shape<kBN, kEpi>;
   if (!tma::bind_context()) return camoe::tm::status(cudaErrorNoDevice);
   CUtensorMap m[6];
   const int ra = kAMN ? 64 : 128, rb = Sh::box(kBMN);
@@ -84,9 +84,9 @@ int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2,
   int64_t pairs = sm_count() / kCG;
   if (pairs < 1) return camoe::tm::status(cudaErrorNoDevice);
   if (2 * tiles < pairs) pairs = tiles > 0 ? 2 * tiles : 1;  // a tile may be done as two halves
-  const auto kernel = gemm_kernel<kCG, kBN, kAMN, kBMN, kMode, kEpi>;
+  const auto kernel = gemm_kernel<kBN, kAMN, kBMN, kMode, kEpi>;
   static std::atomic<uint64_t> opted{0};
-  constexpr int smem = smem_bytes<kCG, kBN, kEpi>();
+  constexpr int smem = smem_bytes<kBN, kEpi>();
   static_assert(smem <= 227 * 1024, "a CTA's shared memory");
   if (const int st = camoe::tm::status(allow_smem(kernel, smem, opted))) return st;
   cudaLaunchConfig_t cfg = {};
@@ -101,7 +101,7 @@ int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2,
   attr[1].val.clusterDim.x = kCG;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = kCG > 1 ? 2 : 1;
+  cfg.numAttrs = 2;
   return camoe::tm::status(cudaLaunchKernelEx(&cfg, kernel, m[0], m[1], m[2], m[3], m[4], m[5], a));
 }
 
@@ -109,10 +109,10 @@ int launch(const Matrix& A, const Matrix& B, const Matrix& A2, const Matrix& B2,
 
 namespace thin {
 
-// CTAs per tile of 128 outputs: as many as keep all of them on the SMs at once (two
-// per SM up to kN = 64), with two pieces of k at least for each
-inline int split_of(int64_t tiles, int64_t K, int per_sm, int least) {
-  const int64_t nk = (K + tc::kBK - 1) / tc::kBK, room = per_sm * tc::sm_count();
+// CTAs per tile of 128 outputs: as many as keep all of them on the SMs at once, two per
+// SM, with two pieces of k at least for each
+inline int split_of(int64_t tiles, int64_t K, int least) {
+  const int64_t nk = (K + tc::kBK - 1) / tc::kBK, room = 2 * tc::sm_count();
   int s = least;
   while (s < 8 && tiles * s * 2 <= room && nk >= 4 * s) s *= 2;
   return s;
@@ -129,7 +129,7 @@ int launch(const void* x, const void* w, Args a, int64_t groups, int64_t row_til
   if (!tma::encode_3d_sw128(&mw, w, a.K, a.O, a.groups, kM) || !tma::encode_3d_sw128(&mx, x, a.K, a.R, 1, kN))
     return camoe::tm::status(cudaErrorInvalidValue);
   const int64_t tiles = (a.O + kM - 1) / kM;
-  a.split = split_of(tiles * groups * row_tiles, a.K, kN <= 64 ? 2 : 1, kEpi == kAdapter ? kN / kAdd : 1);
+  a.split = split_of(tiles * groups * row_tiles, a.K, kEpi == kAdapter ? kN / kAdd : 1);
   const auto kernel = thin_kernel<kN, kEpi>;
   static std::atomic<uint64_t> opted{0};
   if (const int st = camoe::tm::status(tc::allow_smem(kernel, smem_bytes<kN>(kEpi == kAdapter ? 256 : 0), opted)))

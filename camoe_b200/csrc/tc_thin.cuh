@@ -53,7 +53,7 @@ constexpr int kAdapter = 16;  // an epilogue next to those of tc_gemm.cuh
 template <int kN>
 struct Shape {
   static constexpr uint32_t kStage = kWBytes + kN * 128;
-  static constexpr int kFit = (kN <= 64 ? 96 : 160) * 1024 / static_cast<int>(kStage);
+  static constexpr int kFit = 96 * 1024 / static_cast<int>(kStage);  // two CTAs on an SM
   static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
   static constexpr uint32_t kCols = kN < 32 ? 32 : kN;  // tensor-memory columns
 };
@@ -247,7 +247,6 @@ __device__ __forceinline__ void peer_sums(uint32_t part, int r, int split, int r
   }
 }
 
-template <int kN>
 __device__ __forceinline__ void ld_cols(float (&v)[16], uint32_t taddr) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
@@ -397,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 2) thin_kernel(const __grid_constant
         if (c0 >= rows) break;
         float v[16];
         if (k1 > k0) {
-          ld_cols<kN>(v, tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + static_cast<uint32_t>(c0));
+          ld_cols(v, tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + static_cast<uint32_t>(c0));
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e) v[e] = 0.0f;

@@ -63,18 +63,6 @@ bool encode_3d_sw128(CUtensorMap* map, const void* base, int64_t inner, int64_t 
 bool encode_2d_rows(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t rows, int box_bytes,
                     int box_rows);
 
-// Load the box at (x, y, z) of a 3-D map, completing on `bar`.
-__device__ __forceinline__ void load_3d(void* dst_smem, const CUtensorMap* map, int x, int y, int z,
-                                        uint64_t* bar) {
-  const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(dst_smem));
-  const uint32_t mb = static_cast<uint32_t>(__cvta_generic_to_shared(bar));
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(mb)
-      : "memory");
-}
-
 // Load the box at (x, y) of a 2-D map, completing on `bar`.
 __device__ __forceinline__ void load_2d(void* dst_smem, const CUtensorMap* map, int x, int y,
                                         uint64_t* bar) {
