@@ -222,9 +222,9 @@ __global__ void __launch_bounds__(kSortThreads)
     int* temp = first + E + 1;  // [kSortWarps][E + 1]
     int* own = temp + warp * (E + 1);
     for (int i = threadIdx.x; i < kSortWarps * (E + 1); i += kSortThreads) temp[i] = 0;
-    __syncthreads();
     const int64_t cut = blockIdx.x * chunk;
     for (int half = 0; half < 2; ++half) {  // the slots before the chunk, then the others
+      __syncthreads();  // temp is cleared; its sum over the first half is taken before the second adds to it
       const int64_t end = half == 0 ? cut : S;
       for (int64_t t = (half == 0 ? 0 : cut) + warp * 32; t < end; t += 32 * kSortWarps * kSortDeep) {
         int bin[kSortDeep];

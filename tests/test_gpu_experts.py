@@ -89,6 +89,28 @@ def test_dispatch_is_the_stable_sort(N, k, E, empty, dtype):
     assert torch.equal(xs, want)
 
 
+@pytest.mark.parametrize("E", [1, 8, 200, 511, 512])
+@pytest.mark.parametrize("N,k", [(2049, 1), (2048, 2), (8191, 1), (4096, 2), (2731, 3)])
+def test_dispatch_where_each_block_counts_all_slots(N, k, E):
+    """Up to 8192 slots of fewer than 512 experts are placed in one launch, in which a
+    block counts the slots before its chunk and behind it with the same counters:
+    fresh indices each time, spread, skewed and all of one expert."""
+    x = rnd(N, 8, seed=3)
+    for seed in range(4):
+        index = index_of(N, k, E, 200 + seed, 0.0 if seed % 2 else 0.2, torch.int32)
+        if seed == 2:
+            index = torch.where(index > 0, index // 16, index)
+        if seed == 3:
+            index.fill_(E - 1)
+        offsets, position, source = plain_sort(index, E)
+        xs, plan = experts.expert_dispatch(x, index, E)
+        assert plan.offsets.tolist() == offsets
+        assert plan.position.reshape(-1).tolist() == position
+        assert plan.source.tolist() == source
+        used = offsets[-1]
+        assert torch.equal(xs[:used], x[plan.source[:used].long() // k]) and not xs[used:].any()
+
+
 def test_values_outside_the_experts_are_unused():
     index = torch.tensor([[0, 5], [-7, 2], [2 ** 40, 3], [1, -2 ** 40]]).cuda()
     _, plan = experts.expert_dispatch(rnd(4, 8, seed=3), index, 4)
