@@ -11,9 +11,9 @@
 // Many rows (prompts): the rows are sorted by adapter, low = scale (xs down^T) is one
 // grouped product (rounded to bf16, the type of the next product's operand), and
 // the projection's sum runs over [x | low] against [weight | up[a]]: an adapter is
-// D more columns of k for the row tiles that hold rows of it, with zeros in the
-// other rows of the tile (kBlocks and kJoined in tc_gemm.cuh), so row tiles are
-// full whatever the adapters' shares.  The result goes to the row that it came from.
+// D more columns of k for the row tiles that hold rows of it, which add to its own
+// rows only (kBlocks and kJoined in tc_gemm.cuh), so row tiles are full whatever
+// the adapters' shares.  The result goes to the row that it came from.
 #include "camoe_experts.h"
 #include "tc_launch.cuh"
 

@@ -12,8 +12,9 @@
 //   kBlocks: for each group and row tile that share rows a block of the tile's
 //     rows with the group's product in its own rows and zeros in the others;
 //   kJoined: out[p][n] = sum over k of A[p][k] B[n][k] + sum over the groups g of
-//     p's tile of sum over d of block[p][d] B2_g[n][d]: a group's product reaches
-//     its own rows only, as more of the same sum.
+//     p's tile of sum over d of block[p][d] B2_g[n][d].  A group's product leaves
+//     the accumulator's other rows as they are (zeros there would not do: 0 x inf
+//     is NaN, and one group's B2 would reach the rows of the others).
 //
 // One pair of CTAs on two SMs (kCG = 2) per tile of 128 kCG rows x kBN
 // columns, persistent over the tiles:
@@ -206,6 +207,29 @@ __device__ __forceinline__ void mma(uint32_t tmem, uint64_t da, uint64_t db, uin
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem),
         "l"(da), "l"(db), "r"(idesc), "r"(add ? 1u : 0u)
         : "memory");
+}
+// Which of a pair's 256 accumulator rows a product leaves as they are: bit r % 32 of
+// word r / 32 for row r, all but rows [first, end).
+struct Rows {
+  uint32_t off[8];
+  __device__ __forceinline__ void all_but(int first, int end) {
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const int lo = first - 32 * w, hi = end - 32 * w;
+      const uint32_t below = lo <= 0 ? 0u : (lo < 32 ? (1u << lo) - 1u : ~0u);
+      const uint32_t from = hi >= 32 ? 0u : (hi > 0 ? ~0u << hi : ~0u);
+      off[w] = below | from;
+    }
+  }
+};
+// a pair's product that adds to the other rows only
+__device__ __forceinline__ void mma_rows(uint32_t tmem, uint64_t da, uint64_t db, uint32_t idesc, const Rows& r) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, p;\n\t}\n" ::"r"(tmem),
+      "l"(da), "l"(db), "r"(idesc), "r"(r.off[0]), "r"(r.off[1]), "r"(r.off[2]), "r"(r.off[3]), "r"(r.off[4]),
+      "r"(r.off[5]), "r"(r.off[6]), "r"(r.off[7])
+      : "memory");
 }
 // arrive on the barrier (in both CTAs of a pair) once the products issued so far are done
 template <int kCtas>
@@ -578,8 +602,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (done >= 2 && !(ok = warp_wait(&c.acc_empty[b], static_cast<uint32_t>((done / 2 - 1) & 1)))) break;
         fence_after();
       }
-      for (int j = 0; j < x.nk; ++j) {
-        const uint32_t sa = ring0 + s * kStage;
+      // the products of the stage that is next, and what they free
+      const auto stage = [&](bool last, const auto& products) {
+        if (rank == 0) {
+          if (!(ok = warp_wait(&c.full[s], round & 1u))) return;
+          fence_after();
+          if (elect_one()) {
+            products(tmem + static_cast<uint32_t>(b * kBN), ring0 + s * kStage);
+            commit<kCG>(&c.empty[s]);
+            if (last) commit<kCG>(&c.acc_full[b]);
+          }
+          __syncwarp();
+        }
+        if (++s == S) s = 0, ++round;
+      };
+      const auto plain = [&](uint32_t acc, uint32_t sa, bool add) {
+#pragma unroll
+        for (int k = 0; k < kBK / 16; ++k)
+          mma<kCG>(acc, desc<kAMN>(sa + kStep<kAMN> * k), desc<kBMN>(sa + Sh::kABytes + kStep<kBMN> * k), idesc,
+                   add || k > 0);
+      };
+      for (int j = 0; ok && j < x.nk1; ++j) {
         if (kMode == kWeights && tail != 0 && j == x.nk - 1) {
           if (!(ok = warp_wait(&c.tail[s], (tail_phase >> s) & 1u))) break;
           tail_phase ^= 1u << s;
@@ -598,20 +641,29 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
           }
         }
-        if (rank == 0) {
-          if (!(ok = warp_wait(&c.full[s], round & 1u))) break;
-          fence_after();
-          if (elect_one()) {
+        stage(j == x.nk - 1, [&](uint32_t acc, uint32_t sa) { plain(acc, sa, j > 0); });
+      }
+      if (kMode == kJoined) {
+        const int each = (a.K2 + kBK - 1) / kBK, row0 = static_cast<int>(x.row0);
+        const int row1 = x.row1 - x.row0 < Sh::kBM ? static_cast<int>(x.row1) : row0 + Sh::kBM;
+        int group = x.group;
+        for (int j = x.nk1; ok && j < x.nk; ++group) {  // as the producer goes through the groups
+          group = tiles.next_group(group, x.tile);
+          const int first = c.first[group], end = c.first[group + 1];
+          Rows others;
+          others.all_but(first - row0, end - row0);
+          for (int part = 0; ok && part < each; ++part, ++j) {
+            if (first <= row0 && end >= row1)
+              stage(j == x.nk - 1, [&](uint32_t acc, uint32_t sa) { plain(acc, sa, true); });
+            else
+              stage(j == x.nk - 1, [&](uint32_t acc, uint32_t sa) {
 #pragma unroll
-            for (int k = 0; k < kBK / 16; ++k)
-              mma<kCG>(tmem + static_cast<uint32_t>(b * kBN), desc<kAMN>(sa + kStep<kAMN> * k),
-                       desc<kBMN>(sa + Sh::kABytes + kStep<kBMN> * k), idesc, j > 0 || k > 0);
-            commit<kCG>(&c.empty[s]);
-            if (j == x.nk - 1) commit<kCG>(&c.acc_full[b]);
+                for (int k = 0; k < kBK / 16; ++k)
+                  mma_rows(acc, desc<kAMN>(sa + kStep<kAMN> * k), desc<kBMN>(sa + Sh::kABytes + kStep<kBMN> * k),
+                           idesc, others);
+              });
           }
-          __syncwarp();
         }
-        if (++s == S) s = 0, ++round;
       }
       ++done;
     }
@@ -652,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // kBlocks: this lane's row is the group's
       const bool live = kMode != kBlocks || (in_tile + lane >= x.lead && x.row0 + in_tile + lane < x.row1);
       const int rows = left < 32 ? (left > 0 ? static_cast<int>(left) : 0) : 32;
-      const float scale = kEpi == kScale && a.scale != nullptr ? a.scale[x.group] : 1.0f;
+      const float scale = kEpi == kScale && a.scale != nullptr && live ? a.scale[x.group] : 1.0f;
       int to = 0;  // where this lane's row goes
       if (kMode != kWeights && a.scatter != nullptr && lane < rows) to = a.scatter[row0 + lane];
       const int begin = half * (x.width / 2), end = begin + x.width / 2;

@@ -100,6 +100,28 @@ def test_a_row_of_infinities_stays_by_itself(N):
     assert torch.equal(got[keep], clean[keep]) and torch.isnan(got[5]).all()
 
 
+@pytest.mark.parametrize("N,M,D", [(60, 192, 16), (700, 320, 72), (1800, 512, 16)])
+@pytest.mark.parametrize("which", ["up", "down", "scale"])
+def test_an_adapter_that_is_not_finite_reaches_its_own_rows_alone(N, M, D, which):
+    """Rows of several adapters and of none share tiles; one adapter overflowed.  The
+    other rows keep their bits; its own are what the formula gives."""
+    x, w, down, up, adapter, scale = inputs(N, 128, M, D, 5, seed=60)
+    clean = adapters.adapter_linear(x, w, down, up, adapter, scale)
+    broken = {"up": up, "down": down, "scale": scale}
+    bad = broken[which].clone()
+    bad[2].reshape(-1)[:1] = float("inf")
+    bad[2].reshape(-1)[-1:] = float("nan") if which != "scale" else float("inf")
+    broken[which] = bad
+    got = adapters.adapter_linear(x, w, broken["down"], broken["up"], adapter, broken["scale"])
+    own = adapter == 2
+    assert own.any() and torch.equal(got[~own], clean[~own])
+    if which == "up":  # the first output row of up holds the infinity, the last the NaN
+        assert not torch.isfinite(got[own][:, 0]).any() and torch.isnan(got[own][:, -1]).all()
+        assert torch.equal(got[own][:, 1:-1], clean[own][:, 1:-1])
+    else:
+        assert not torch.isfinite(got[own]).any()
+
+
 def test_empty_and_another_stream():
     x, w, down, up, adapter, scale = inputs(500, 128, 256, 16, 5, seed=30)
     first = adapters.adapter_linear(x, w, down, up, adapter, scale)
