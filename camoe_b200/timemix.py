@@ -55,6 +55,11 @@ def _p(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+def _f32(t):
+    """A parameter as the kernels read it: fp32, whatever the module was converted to."""
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
+
+
 def _stream(t):
     return torch.cuda.current_stream(t.device).cuda_stream
 
@@ -163,7 +168,7 @@ class Mix6Fn(torch.autograd.Function):
 class Wkv7BlockFn(torch.autograd.Function):
     """prep -> WKV-7 op -> (post, lnsa) between the projection GEMMs and the
     output GEMM.  Inputs are [B, T, C] bf16 activations (vl and v_first None
-    for layer 0) and fp32 parameters; returns (z, state_representation)."""
+    for layer 0) and parameters (used in fp32); returns (z, state_representation)."""
 
     @staticmethod
     def forward(ctx, r, wl, k, v, vl, al, v_first, g, prep_par, r_k, lnx_w, lnx_b, lnsa_w,
@@ -172,6 +177,8 @@ class Wkv7BlockFn(torch.autograd.Function):
         H = C // HEAD_SIZE
         acts = [t.contiguous() if t is not None else None for t in (r, wl, k, v, vl, al, v_first, g)]
         r, wl, k, v, vl, al, v_first, g = acts
+        prep_par, r_k, lnx_w, lnx_b, lnsa_w, lnsa_b = (
+            _f32(t) for t in (prep_par, r_k, lnx_w, lnx_b, lnsa_w, lnsa_b))
         L = _lib.lib()
         dev = r.device
         op_in = [torch.empty(B, T, C, dtype=_BF, device=dev) for _ in range(5)]

@@ -88,6 +88,54 @@ def test_block_trains_and_generates_the_same_steps():
     assert nrel(torch.cat(outs, 1).cpu(), y.detach().cpu()) < 2e-2
 
 
+def in_bf16(module):
+    """(the module in fp32 with values that bf16 holds, the module in bf16)"""
+    import copy
+    low = copy.deepcopy(module).bfloat16()
+    return copy.deepcopy(low).float(), low
+
+
+@pytest.mark.parametrize("layer", [0, 1])
+def test_a_time_mix_in_bf16_is_the_same_with_those_values(layer):
+    """The kernels take fp32 parameters and the products bf16 ones: which of both the
+    module holds is no difference, but that its gradients are rounded."""
+    B, T, C = 2, 48, 128
+    full, low = in_bf16(block(C, layer=layer, seed=5).att)
+    x = torch.randn(B, T, C, device="cuda")
+    v_first = torch.randn(B, T, C, device="cuda").bfloat16() if layer else None
+    got = []
+    for m in (full, low):
+        xs = x.clone().requires_grad_()
+        y, _, srep = m(xs, v_first)
+        (y.float().square().sum() + srep.square().sum()).backward()
+        got.append((y, srep, xs.grad, {n: p.grad for n, p in m.named_parameters()}))
+    for a, b in zip(got[0][:3], got[1][:3]):
+        assert torch.equal(a, b)
+    for n, g in got[0][3].items():
+        assert (g is None) == (got[1][3][n] is None), n
+        if g is not None:
+            assert got[1][3][n].dtype == torch.bfloat16 and torch.equal(g.bfloat16(), got[1][3][n]), n
+    with torch.no_grad():
+        for m in (full, low):
+            y, _, srep, _ = m.forward_state(x, v_first)
+            got.append((y, srep))
+    assert torch.equal(got[2][0], got[3][0]) and torch.equal(got[2][1], got[3][1])
+
+
+@pytest.mark.parametrize("tokens", [1, 900])
+def test_an_expert_layer_in_bf16_is_the_same_with_those_values(tokens):
+    full, low = in_bf16(block(64, seed=6, n_experts=5, hidden=160).experts)
+    x = torch.randn(tokens, 64, device="cuda").bfloat16()
+    index = torch.randint(-1, 5, (tokens, 2), device="cuda")
+    weight = torch.rand(tokens, 2, device="cuda")
+    dout = torch.randn(tokens, 64, device="cuda").bfloat16()
+    a, b = full(x, index, weight), low(x, index, weight)
+    assert torch.equal(a, b)
+    for p, q in zip(torch.autograd.grad(a, (full.w_up, full.w_down), dout),
+                    torch.autograd.grad(b, (low.w_up, low.w_down), dout)):
+        assert q.dtype == torch.bfloat16 and torch.equal(p.bfloat16(), q)
+
+
 @pytest.mark.parametrize("T", [1, 300])
 def test_adapters_are_the_weights_they_amount_to(T):
     B, C, L, D = 3, 128, 2, 8
