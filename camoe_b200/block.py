@@ -37,8 +37,9 @@ class ExpertBlock(nn.Module):
         return self.experts(h, index, torch.softmax(value, dim=-1))
 
     def forward(self, x: torch.Tensor, v_first: torch.Tensor | None = None):
-        """x [B, T, C] fp32.  Returns (x, v_first, state_representation)."""
-        y, v_first, srep = self.att(self.ln1(x), v_first)
+        """x [B, T, C] fp32 or bf16, whose dtype the result has.  Returns (x, v_first,
+        state_representation)."""
+        y, v_first, srep = self.att(self.ln1(x.to(self.ln1.weight.dtype)), v_first)
         x = x + y.to(x.dtype)
         return x + self._experts(x).to(x.dtype), v_first, srep
 
