@@ -172,6 +172,14 @@ inline int64_t chunk_of(int64_t S) {
 // Whether each block counts all slots itself, one launch less, where its counters fit.
 // Kernel times: 7001 slots 6.0 us, 3.3 + 4.6 in two launches; 16384 slots 10.7 us, 3.1 + 4.3.
 inline bool alone(int64_t S, int64_t E) { return S <= 8192 && E < 512; }
+// Shared memory of place_kernel, and the most that any call asks for: the limit is set
+// to that one, so that host threads with sorts of different sizes do not lower each
+// other's before a launch.
+constexpr int place_smem(bool solo, int E) {
+  return ((solo ? 2 : 1) * kSortWarps + 2) * (E + 1) * static_cast<int>(sizeof(int));
+}
+constexpr int kPlaceSmem = place_smem(false, kMaxExperts) > place_smem(true, 511) ? place_smem(false, kMaxExperts)
+                                                                                  : place_smem(true, 511);
 inline int64_t chunks_of(int64_t S) { return (S + chunk_of(S) - 1) / chunk_of(S); }
 
 // slots of each expert in each chunk: counts[chunk][expert]
@@ -521,10 +529,10 @@ int sort(const P* x, const I* index, P* xs, int* offsets, int* position, int* so
     count_kernel<I><<<g, kSortThreads, 0, st>>>(index, work, S, chunk, E);
     if (const int e = camoe::tm::status(cudaGetLastError())) return e;
   }
-  const int smem = ((solo ? 2 : 1) * kSortWarps + 2) * (E + 1) * static_cast<int>(sizeof(int));
+  const int smem = place_smem(solo, E);
   const auto place = place_kernel<I, kKeep>;
   if (smem > 48 * 1024)
-    if (const int e = camoe::tm::status(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))
+    if (const int e = camoe::tm::status(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, kPlaceSmem)))
       return e;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

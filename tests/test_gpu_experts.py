@@ -379,6 +379,35 @@ def test_gradients_that_are_strided_or_off_alignment():
     assert torch.equal(a, b)
 
 
+def test_sorts_of_different_sizes_from_two_host_threads():
+    """Through the C ABI, whose calls run side by side: sorts that need different amounts
+    of shared memory."""
+    import threading
+    lib, failed = _lib.lib(), []
+
+    def sorts(N, E, stream):
+        index = index_of(N, 1, E, 110, 0.1, torch.int32)
+        offsets, position, source = (torch.empty(n, dtype=torch.int32, device="cuda") for n in (E + 1, N, N))
+        need = lib.camoe_ex_dispatch_work_bytes(N, 1, E)
+        work = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        for _ in range(3000):
+            status = lib.camoe_ex_dispatch(None, 0, index.data_ptr(), 4, None, offsets.data_ptr(), position.data_ptr(),
+                                           source.data_ptr(), work.data_ptr(), need, N, 1, E, 8, stream.cuda_stream)
+            if status:
+                return failed.append(status)
+        stream.synchronize()
+        if [offsets.tolist(), position.tolist(), source.tolist()] != list(plain_sort(index, E)):
+            failed.append("wrong")
+
+    threads = [threading.Thread(target=sorts, args=(N, E, torch.cuda.Stream())) for N, E in ((9000, 1024), (9000, 800))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+
+
 def test_empty_inputs():
     offsets = torch.zeros(4, dtype=torch.int32, device="cuda")
     w_up, w_down = rnd(3, 16, 8, seed=60), rnd(3, 8, 16, seed=61)
