@@ -31,7 +31,7 @@ def _refuse(x, weight, down, up, adapter, scale):
     _check(adapter, "adapter", (N,), torch.int32, dev)
     if scale is not None:
         _check(scale, "scale", (L,), torch.float32, dev)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, weight, down, up)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, down, up, scale)):
         raise RuntimeError("adapter_linear has no backward: call it under torch.no_grad()")
     _check_aligned(x, weight, down, up)
     raise ValueError(f"C, M and D must be positive multiples of 8, D at most {MAX_RANK}, 1 to {MAX_ADAPTERS} "

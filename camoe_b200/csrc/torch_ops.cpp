@@ -214,7 +214,7 @@ py::object adapter_linear(const Tensor& x, const Tensor& weight, const Tensor& d
       !fits(down, {L, D, C}, torch::kBFloat16, device) || !fits(up, {L, M, D}, torch::kBFloat16, device) ||
       !fits(adapter, {N}, torch::kInt32, device) || (scale && !fits(*scale, {L}, torch::kFloat32, device)) ||
       C < 8 || M < 8 || D < 8 || C % 8 != 0 || M % 8 != 0 || D % 8 != 0 || D > 256 || L < 1 || L > 1024 ||
-      !aligned({&x, &weight, &down, &up}) || wants_grad({&x, &weight, &down, &up}))
+      !aligned({&x, &weight, &down, &up}) || wants_grad({&x, &weight, &down, &up}) || (scale && wants_grad({&*scale})))
     return py::none();
   const c10::cuda::CUDAGuard guard(device);
   Tensor y = at::empty({N, M}, x.options());

@@ -153,3 +153,11 @@ def test_refusals():
             call(*args)
     with torch.no_grad():
         call(x, w.clone().requires_grad_(), down, up, adapter, scale)
+
+
+def test_a_trainable_scale_is_refused_as_the_other_inputs_are():
+    x, w, down, up, adapter, scale = inputs(4, 64, 32, 8, 2, seed=41)
+    with pytest.raises(RuntimeError, match="no backward"):
+        adapters.adapter_linear(x, w, down, up, adapter, scale.requires_grad_())
+    with torch.no_grad():
+        adapters.adapter_linear(x, w, down, up, adapter, scale)
