@@ -44,6 +44,11 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (t->requires_grad()) return true;
   return false;
 }
+// Forward-mode tangents, which the kernels would drop.
+void no_tangents(const char* call, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), call, " has no forward-mode derivative");
+}
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor bytes(size_t n, const Tensor& like) {
   return n > 0 ? at::empty({static_cast<int64_t>(n)}, like.options().dtype(torch::kUInt8)) : Tensor();
@@ -103,6 +108,7 @@ py::object dispatch(const Tensor& x, const Tensor& index, int64_t E) {
       index.device() != x.device() || index.size(0) != x.size(0) || E < 1 || E > 1024 || index.size(1) < 1 ||
       index.size(1) > 64)
     return py::none();
+  no_tangents("expert_dispatch", {&x});
   Sorted r;
   if (wants_grad({&x}))
     r.xs = DispatchFn::apply(x, index, E, &r);
@@ -145,6 +151,7 @@ py::object combine(const Tensor& ys, const Tensor& weight, const Tensor& offsets
       !fits(position, {N, k}, torch::kInt32, device) ||
       !fits(offsets, {offsets.size(0)}, torch::kInt32, device) || !fits(source, {N * k}, torch::kInt32, device))
     return py::none();
+  no_tangents("expert_combine", {&ys, &weight});
   return py::cast(wants_grad({&ys, &weight}) ? CombineFn::apply(ys, weight, offsets, position)
                                              : sum_rows(ys, weight, position));
 }
@@ -199,6 +206,7 @@ py::object ffn(const Tensor& xs, const Tensor& w_up, const Tensor& w_down, const
       !fits(w_down, {E, C, F}, torch::kBFloat16, device) || !fits(offsets, {E + 1}, torch::kInt32, device) ||
       E < 1 || E > 1024 || C < 8 || F < 8 || C % 8 != 0 || F % 8 != 0 || !aligned({&xs, &w_up, &w_down}))
     return py::none();
+  no_tangents("expert_ffn", {&xs, &w_up, &w_down});
   return py::cast(wants_grad({&xs, &w_up, &w_down}) ? FfnFn::apply(xs, w_up, w_down, offsets)
                                                     : ffn_forward(xs, w_up, w_down, offsets, false).ys);
 }
@@ -216,6 +224,8 @@ py::object adapter_linear(const Tensor& x, const Tensor& weight, const Tensor& d
       C < 8 || M < 8 || D < 8 || C % 8 != 0 || M % 8 != 0 || D % 8 != 0 || D > 256 || L < 1 || L > 1024 ||
       !aligned({&x, &weight, &down, &up}) || wants_grad({&x, &weight, &down, &up}) || (scale && wants_grad({&*scale})))
     return py::none();
+  no_tangents("adapter_linear", {&x, &weight, &down, &up});
+  if (scale) no_tangents("adapter_linear", {&*scale});
   const c10::cuda::CUDAGuard guard(device);
   Tensor y = at::empty({N, M}, x.options());
   const size_t need = camoe_ad_work_bytes(N, C, M, D, L);

@@ -450,3 +450,29 @@ def test_refusals():
     for kind, call in bad:
         with pytest.raises(kind):
             call()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused_not_dropped(grad):
+    """Forward-mode derivatives, with and without a gradient wanted as well."""
+    import torch.autograd.forward_ad as fw
+    from camoe_b200 import adapters
+    x, index = rnd(4, 16, seed=120), torch.zeros(4, 2, dtype=torch.int64, device="cuda")
+    xs, plan = experts.expert_dispatch(x, index, 3)
+    w = torch.ones(4, 2, device="cuda")
+    w_up, w_down = rnd(3, 32, 16, seed=121), rnd(3, 16, 32, seed=122)
+    down, up, which = rnd(2, 8, 16, seed=123), rnd(2, 32, 8, seed=124), torch.zeros(4, dtype=torch.int32, device="cuda")
+    scale = torch.ones(2, device="cuda")
+    calls = [
+        (lambda a: experts.expert_dispatch(a, index, 3), (x,)),
+        (lambda a, b: experts.expert_combine(a, b, plan), (xs, w)),
+        (lambda a, b, c: experts.expert_ffn(a, b, c, plan.offsets), (xs, w_up, w_down)),
+        (lambda a, b, c, d, e: adapters.adapter_linear(a, b, c, d, which, e), (x, w_up[0], down, up, scale)),
+    ]
+    for call, args in calls:
+        for i in range(len(args)):
+            with fw.dual_level(), torch.set_grad_enabled(grad and len(args) < 5):
+                dual = fw.make_dual(args[i], torch.ones_like(args[i]))
+                other = [t.clone().requires_grad_(grad and len(args) < 5) for t in args]
+                with pytest.raises(RuntimeError, match="forward"):
+                    call(*[dual if j == i else t for j, t in enumerate(other)])
