@@ -60,6 +60,24 @@ Tensor packed(const Tensor& g) {
   return aligned({&t}) ? t : t.clone();
 }
 
+// A gradient of a backward that is recorded (create_graph): the kernels have no
+// derivative of it, so going back through it is an error.  from: what it depends on.
+struct Once : torch::autograd::Function<Once> {
+  static Tensor forward(AutogradContext*, const Tensor& gradient, const Tensor&) { return gradient.detach(); }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "the expert layer's operators are differentiable once: their gradients have no gradient");
+    return {};
+  }
+};
+void once(Tensor& gradient, std::initializer_list<const Tensor*> from) {
+  if (!at::GradMode::is_enabled() || !gradient.defined()) return;
+  for (const Tensor* t : from)
+    if (t->requires_grad()) {
+      gradient = Once::apply(gradient, *t);
+      return;
+    }
+}
+
 // ---- tokens to their experts and back
 
 struct Sorted {
@@ -96,9 +114,11 @@ struct DispatchFn : torch::autograd::Function<DispatchFn> {
     return plan->xs;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    Tensor dx;
-    if (grads[0].defined()) dx = sum_rows(packed(grads[0]), Tensor(), ctx->get_saved_variables()[0]);
-    return {dx, Tensor(), Tensor(), Tensor()};
+    variable_list out(4);
+    if (!grads[0].defined()) return out;
+    out[0] = sum_rows(packed(grads[0]), Tensor(), ctx->get_saved_variables()[0]);
+    once(out[0], {&grads[0]});
+    return out;
   }
 };
 
@@ -136,6 +156,8 @@ struct CombineFn : torch::autograd::Function<CombineFn> {
                                offsets.data_ptr<int32_t>(), position.data_ptr<int32_t>(), ptr(out[0]),
                                static_cast<float*>(ptr(out[1])), position.size(0), position.size(1),
                                offsets.size(0) - 1, ys.size(1), stream_of(ys)));
+    once(out[0], {&grads[0], &weight});
+    once(out[1], {&grads[0], &ys});
     return out;
   }
 };
@@ -194,6 +216,8 @@ struct FfnFn : torch::autograd::Function<FfnFn> {
                            offsets.data_ptr<int32_t>(), h.data_ptr(), ptr(saved[5]), ptr(dpre), ptr(out[0]),
                            ptr(out[1]), ptr(out[2]), xs.size(0), w_up.size(0), xs.size(1), w_up.size(1),
                            stream_of(xs)));
+    for (int i = 0; i < 2; ++i) once(out[i], {&grads[0], &xs, &w_up, &w_down});
+    once(out[2], {&grads[0], &xs, &w_up});
     return out;
   }
 };

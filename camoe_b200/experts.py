@@ -10,8 +10,8 @@ back to their tokens with their weights:
     ys = expert_ffn(xs, w_up, w_down, plan.offsets)   # w_up [E, F, C], w_down [E, C, F]
     out = expert_combine(ys, weight, plan)            # weight [N, k] fp32
 
-All three are differentiable (the index is not) and launch on the current CUDA
-stream without synchronising.  A slot whose index is outside [0, n_experts) is
+All three are differentiable once, in reverse mode (the index is not), and launch
+on the current CUDA stream without synchronising.  A slot whose index is outside [0, n_experts) is
 unused: it reads nothing and contributes nothing, and a token without used
 slots gets zeros.  ``ExpertLayer`` is the module over them.  The C ABI is
 include/camoe_experts.h.

@@ -476,3 +476,39 @@ def test_tangents_are_refused_not_dropped(grad):
                 other = [t.clone().requires_grad_(grad and len(args) < 5) for t in args]
                 with pytest.raises(RuntimeError, match="forward"):
                     call(*[dual if j == i else t for j, t in enumerate(other)])
+
+
+def test_second_derivatives_are_refused_not_dropped():
+    """A gradient that was recorded takes part in another backward: an error, also where
+    the loss reaches the inputs by another way.  Recorded and not gone through again
+    it is the gradient."""
+    N, k, E, C, F = 40, 2, 3, 16, 32
+    index = index_of(N, k, E, 130, 0.1)
+    x, ys = rnd(N, C, seed=131).requires_grad_(), rnd(N * k, C, seed=132).requires_grad_()
+    w = rnd(N, k, seed=133, dtype=F32).requires_grad_()
+    w_up, w_down = rnd(E, F, C, seed=134).requires_grad_(), rnd(E, C, F, seed=135).requires_grad_()
+    plan = experts.expert_dispatch(x.detach(), index, E)[1]
+    for call, ins in (
+        (lambda: experts.expert_dispatch(x, index, E)[0], (x,)),
+        (lambda: experts.expert_combine(ys, w, plan), (ys, w)),
+        (lambda: experts.expert_ffn(ys, w_up, w_down, plan.offsets), (ys, w_up, w_down)),
+    ):
+        out = call()
+        dout = torch.ones_like(out).requires_grad_()
+        want = torch.autograd.grad(call(), ins, dout.detach())
+        got = torch.autograd.grad(out, ins, dout, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        for g in got:
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                (g.float().square().sum() + ins[0].float().sum() + dout.float().sum()).backward(retain_graph=True)
+    # a weight as the only way to what the gradient depends on
+    out = experts.expert_combine(ys, w, plan)
+    dys, = torch.autograd.grad(out, ys, torch.ones_like(out), create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (dys.float().sum() + w.sum()).backward()
+    # a gradient that depends on constants alone: nothing to refuse
+    dys, = torch.autograd.grad(experts.expert_combine(ys, w.detach(), plan), ys, torch.ones_like(out), create_graph=True)
+    assert not dys.requires_grad
+    out = experts.expert_dispatch(x, index, E)[0]
+    dx, = torch.autograd.grad(out, x, torch.ones_like(out), create_graph=True)
+    assert not dx.requires_grad
