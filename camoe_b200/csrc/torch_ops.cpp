@@ -165,11 +165,11 @@ struct CombineFn : torch::autograd::Function<CombineFn> {
 py::object combine(const Tensor& ys, const Tensor& weight, const Tensor& offsets, const Tensor& position,
                    const Tensor& source) {
   if (!ys.is_cuda() || ys.dim() != 2 || !is_float(ys) || !ys.is_contiguous() || position.dim() != 2 ||
-      offsets.dim() != 1 || offsets.size(0) < 2)
+      offsets.dim() != 1 || offsets.size(0) < 2 || offsets.size(0) > 1025)
     return py::none();
   const int64_t N = position.size(0), k = position.size(1);
   const auto device = ys.device();
-  if (ys.size(0) != N * k || !fits(weight, {N, k}, torch::kFloat32, device) ||
+  if (k < 1 || k > 64 || ys.size(0) != N * k || !fits(weight, {N, k}, torch::kFloat32, device) ||
       !fits(position, {N, k}, torch::kInt32, device) ||
       !fits(offsets, {offsets.size(0)}, torch::kInt32, device) || !fits(source, {N * k}, torch::kInt32, device))
     return py::none();

@@ -99,6 +99,7 @@ def _refuse_combine(ys, weight, plan):
     _check(weight, "weight", (N, k), torch.float32, ys.device)
     for name, shape in (("offsets", plan.offsets.shape), ("position", (N, k)), ("source", (N * k,))):
         _check(getattr(plan, name), f"plan.{name}", shape, torch.int32, ys.device)
+    raise ValueError(f"1 to {MAX_EXPERTS} experts and 1 to {MAX_SLOTS} slots per token, got {plan.offsets.shape[0] - 1} and {k}")
 
 
 def expert_combine(ys: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:

@@ -512,3 +512,18 @@ def test_second_derivatives_are_refused_not_dropped():
     out = experts.expert_dispatch(x, index, E)[0]
     dx, = torch.autograd.grad(out, x, torch.ones_like(out), create_graph=True)
     assert not dx.requires_grad
+
+
+def test_combine_refuses_what_its_backward_could_not_take():
+    """The limits of the sort, before the forward rather than in the backward."""
+    def call(N, k, E):
+        plan = experts.ExpertPlan(torch.zeros(E + 1, dtype=torch.int32, device="cuda"),
+                                  torch.full((N, k), -1, dtype=torch.int32, device="cuda"),
+                                  torch.full((N * k,), -1, dtype=torch.int32, device="cuda"))
+        ys = torch.zeros(N * k, 8, device="cuda").requires_grad_()
+        return ys, experts.expert_combine(ys, torch.zeros(N, k, device="cuda"), plan)
+    for N, k, E in ((4, 2, 1025), (4, 65, 8), (4, 0, 8)):
+        with pytest.raises(ValueError, match="experts and 1 to 64 slots"):
+            call(N, k, E)
+    ys, out = call(4, 64, 1024)
+    assert not torch.autograd.grad(out.sum(), ys)[0].any() and not out.any()
