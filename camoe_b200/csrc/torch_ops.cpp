@@ -14,6 +14,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <stdexcept>
+#include <string>
+
 #include "camoe_experts.h"
 
 extern "C" const char* camoe_wkv7_strerror(int code);
@@ -24,8 +27,15 @@ using torch::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// A non-zero status of the C ABI; camoe_b200._lib raises it as its CamoeError (out of
+// a backward torch turns it into a plain RuntimeError).
+struct Status : std::runtime_error {
+  int code;
+  explicit Status(int c)
+      : std::runtime_error("camoe_wkv7 error " + std::to_string(c) + ": " + camoe_wkv7_strerror(c)), code(c) {}
+};
 void check(int status) {
-  TORCH_CHECK(status == 0, "camoe_wkv7 error ", status, ": ", camoe_wkv7_strerror(status));
+  if (status != 0) throw Status(status);
 }
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 int dtype_of(const Tensor& t) { return t.scalar_type() == torch::kBFloat16 ? 0 : 1; }
@@ -263,6 +273,17 @@ py::object adapter_linear(const Tensor& x, const Tensor& weight, const Tensor& d
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  py::register_exception_translator([](std::exception_ptr p) {
+    try {
+      std::rethrow_exception(p);
+    } catch (const Status& e) {
+      try {
+        py::module_::import("camoe_b200._lib").attr("check")(e.code);
+      } catch (py::error_already_set& raised) {
+        raised.restore();
+      }
+    }
+  });
   m.def("dispatch", &dispatch);
   m.def("combine", &combine);
   m.def("ffn", &ffn);

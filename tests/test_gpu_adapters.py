@@ -161,3 +161,13 @@ def test_a_trainable_scale_is_refused_as_the_other_inputs_are():
         adapters.adapter_linear(x, w, down, up, adapter, scale.requires_grad_())
     with torch.no_grad():
         adapters.adapter_linear(x, w, down, up, adapter, scale)
+
+
+def test_a_status_of_the_library_is_its_own_error():
+    """A width that only the library refuses, before any launch."""
+    C = (1 << 24) + 8
+    x, w, down = (torch.zeros(*s, C, dtype=BF, device="cuda") for s in ((1,), (8,), (1, 8)))
+    with pytest.raises(_lib.CamoeError) as e:
+        adapters.adapter_linear(x, w, down, torch.zeros(1, 8, 8, dtype=BF, device="cuda"),
+                                torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert e.value.status == _lib.ERR_SHAPE
