@@ -349,8 +349,8 @@ class RWKV7TimeMix(nn.Module):
 
         ``adapters`` (an ``adapters.AdapterSet`` with any of "receptance", "key",
         "value" and "output") adds to each of those projections the low-rank
-        adapter of each sequence's request: ``adapter`` [B] int32, a sequence
-        outside [0, L) has none."""
+        adapter of each sequence's request: ``adapter`` [B] int32 or int64, a
+        sequence outside [0, L) has none."""
         B, T, C = x.shape
         H = C // HEAD_SIZE
         dev = x.device
@@ -377,8 +377,13 @@ class RWKV7TimeMix(nn.Module):
             lin = (lambda name, t: F.linear(t, W(getattr(self, name))))
         else:
             if adapter is None or tuple(adapter.shape) != (B,):
-                raise ValueError(f"adapters need the adapter of each sequence, [B] = [{B}] int32")
-            of_row = adapter.to(torch.int32).repeat_interleave(T) if T > 1 else adapter.to(torch.int32).contiguous()
+                raise ValueError(f"adapters need the adapter of each sequence, [B] = [{B}] int32 or int64")
+            if adapter.is_floating_point() or adapter.dtype == torch.bool:
+                raise TypeError(f"adapter has dtype {adapter.dtype}, expected int32 or int64")
+            if adapter.dtype == torch.int64:  # ids beyond int32 stay outside [0, L)
+                adapter = adapter.clamp(-1, 2 ** 31 - 1)
+            adapter = adapter.to(torch.int32)
+            of_row = adapter.repeat_interleave(T) if T > 1 else adapter.contiguous()
             lin = (lambda name, t: adapters.linear(name, t, W(getattr(self, name)).contiguous(), of_row))
         r = lin("receptance", xr).contiguous()
         k = lin("key", xk).contiguous()

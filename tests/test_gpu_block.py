@@ -193,6 +193,23 @@ def test_adapters_are_the_weights_they_amount_to(T):
         b.forward_state(x, adapters=adapters)
 
 
+@pytest.mark.parametrize("T", [1, 5])
+def test_ids_of_adapters_are_taken_as_they_are(T):
+    """64-bit ids whose low 32 bits are an adapter's are outside [0, L): no adapter; ids
+    of another kind than whole numbers are refused."""
+    B, C = 3, 128
+    b = block(C, seed=8).att
+    x = torch.randn(B, T, C, device="cuda")
+    adapters = AdapterSet().add("key", torch.randn(2, 8, C, device="cuda"), torch.randn(2, C, 8, device="cuda"))
+    run = lambda ids, dtype: b.forward_state(x, adapters=adapters, adapter=torch.tensor(ids, dtype=dtype, device="cuda"))[0]
+    want = run([-1, 1, -1], torch.int32)
+    assert torch.equal(run([2 ** 32, 1, -2 ** 32 + 1], torch.int64), want)
+    assert torch.equal(run([-1, 1, -1], torch.int8), want)
+    for dtype in (torch.float32, torch.bool):
+        with pytest.raises(TypeError):
+            run([0, 1, 0], dtype)
+
+
 def test_the_example_runs():
     from camoe_b200 import block as module
     module.main()
