@@ -153,6 +153,7 @@ int camoe_ad_linear(const void* x, const void* weight, const void* down, const v
     if (p == nullptr) return 1;
   for (const void* p : {x, weight, down, up, static_cast<const void*>(y), static_cast<const void*>(work)})
     if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0) return 4;
+  if ((reinterpret_cast<uintptr_t>(adapter) | reinterpret_cast<uintptr_t>(scale)) % 4 != 0) return 4;
   const Layout w = layout(N, C, M, D, L);
   if (work_bytes < w.total) return 5;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -105,7 +105,7 @@ int camoe_ex_ffn_fwd(const void* xs, const void* w_up, const void* w_down, const
   if (const int st = check(offsets, R, E, C, F)) return st;
   if (R == 0) return 0;
   if (xs == nullptr || w_up == nullptr || w_down == nullptr || h == nullptr || ys == nullptr) return 1;
-  if (!aligned(xs, w_up, w_down, h, h_low, ys)) return 4;
+  if (!aligned(xs, w_up, w_down, h, h_low, ys) || reinterpret_cast<uintptr_t>(offsets) % 4 != 0) return 4;
   int8_t* low = static_cast<int8_t*>(h_low);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (few_rows(R, E)) {
@@ -129,7 +129,9 @@ int camoe_ex_ffn_bwd(const void* dys, const void* xs, const void* w_up, const vo
   using namespace camoe;
   using namespace camoe::ffn;
   if (const int st = check(offsets, R, E, C, F)) return st;
-  if (!aligned(dys, xs, w_up, w_down, h, h_low, dpre, dxs, dw_up, dw_down)) return 4;
+  if (!aligned(dys, xs, w_up, w_down, h, h_low, dpre, dxs, dw_up, dw_down) ||
+      reinterpret_cast<uintptr_t>(offsets) % 4 != 0)
+    return 4;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (R == 0) {
     const size_t bytes = static_cast<size_t>(E * C * F) * sizeof(bf16);

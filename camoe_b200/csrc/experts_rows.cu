@@ -506,6 +506,14 @@ int64_t pieces(int64_t C, int size, Ptr... p) {
   return (C * size) % 16 == 0 && (all & 15u) == 0 ? C * size / 16 : 0;
 }
 
+// whether all pointers are at multiples of `size` bytes
+template <typename... Ptr>
+bool at_multiples(int size, Ptr... p) {
+  uintptr_t all = 0;
+  ((all |= reinterpret_cast<uintptr_t>(p)), ...);
+  return all % static_cast<uintptr_t>(size) == 0;
+}
+
 int check(int64_t N, int64_t k, int64_t E, int64_t C, int dtype) {
   if (dtype != 0 && dtype != 1) return 2;
   if (N < 0 || k < 1 || E < 1 || C < 0) return 1;
@@ -633,10 +641,14 @@ int camoe_ex_dispatch(const void* x, int dtype, const void* index, int index_byt
   if (const int st = check(N, k, E, C, dtype)) return st;
   if (index_bytes != 4 && index_bytes != 8) return 2;
   if (offsets == nullptr) return 1;
+  if (!at_multiples(4, offsets)) return 4;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (N == 0)
     return camoe::tm::status(cudaMemsetAsync(offsets, 0, static_cast<size_t>(E + 1) * sizeof(int), s));
   if (index == nullptr || position == nullptr || source == nullptr || (xs != nullptr && x == nullptr)) return 1;
+  if (!at_multiples(dtype == 0 ? 2 : 4, x, xs) || !at_multiples(index_bytes, index) ||
+      !at_multiples(4, offsets, position, source, work))
+    return 4;
   const size_t need = sort_bytes(N, k, E);
   if (need > 0 && work == nullptr) return 1;
   if (work_bytes < need) return 5;
@@ -656,6 +668,7 @@ int camoe_ex_combine(const void* in, int dtype, const float* weight, const int32
   if (const int st = check(N, k, 1, C, dtype)) return st;
   if (N == 0 || C == 0) return 0;
   if (in == nullptr || position == nullptr || out == nullptr) return 1;
+  if (!at_multiples(dtype == 0 ? 2 : 4, in, out) || !at_multiples(4, weight, position)) return 4;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int kk = static_cast<int>(k);
   const int64_t V = pieces(C, dtype == 0 ? 2 : 4, in, out);
@@ -675,6 +688,7 @@ int camoe_ex_combine_bwd(const void* dout, int dtype, const void* ys, const floa
   if (N == 0 || (dys == nullptr && dweight == nullptr)) return 0;
   if (position == nullptr || weight == nullptr || (dys != nullptr && offsets == nullptr)) return 1;
   if (C > 0 && (dout == nullptr || (dweight != nullptr && ys == nullptr))) return 1;
+  if (!at_multiples(dtype == 0 ? 2 : 4, dout, ys, dys) || !at_multiples(4, weight, offsets, position, dweight)) return 4;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int kk = static_cast<int>(k), e = static_cast<int>(E);
   const int64_t V = pieces(C, dtype == 0 ? 2 : 4, dout, ys, dys);

@@ -18,7 +18,8 @@
  * All three are int32, so R is at most 2^31 - 1.  dtype is 0 (bf16) or 1
  * (fp32); arithmetic is fp32.  All arrays are contiguous; those of the products
  * and adapters are 16-byte aligned, those of the sort, the copies and the sums
- * need their element's alignment (and are fastest at 16 bytes).  Calls are
+ * need their element's alignment (and are fastest at 16 bytes); other addresses
+ * are refused.  Calls are
  * asynchronous on `stream`, allocate nothing, and return the status codes of
  * camoe_wkv7.h (0 = ok).  1 <= E <= 1024, 1 <= k <= 64.
  */

@@ -99,3 +99,29 @@ def test_python_refuses_cpu_tensors():
                                                  torch.zeros(4, dtype=torch.int32))):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+def test_addresses_off_their_elements_are_refused():
+    """Every array of every call, one element's half or less beside its place."""
+    lib, want = _lib.lib(), _lib.ERR_ALIGNMENT
+    f, b, p = lib.camoe_ex_combine, lib.camoe_ex_combine_bwd, lib.camoe_ex_dispatch
+    for dtype, off in ((0, 1), (1, 2)):
+        for at, o in ((0, off), (2, off), (3, 2), (4, 2), (5, 2), (6, 2), (7, 2)):
+            arrays = [P, P, P, P, P, P, P, P]  # x, index, xs, offsets, position, source, work; the last unused
+            if at == 7:
+                arrays[1] += 4
+            else:
+                arrays[at] += o
+            x, index, xs, offsets, position, source, work, _ = arrays
+            assert p(x, dtype, index, 8, xs, offsets, position, source, work, 1 << 20, 50, 2, 8, 16, None) == want, at
+        for at, o in ((0, off), (1, 2), (2, 2), (3, off)):
+            rows, weight, position, out = [P + (o if i == at else 0) for i in range(4)]
+            assert f(rows, dtype, weight, position, out, 4, 2, 16, None) == want, at
+        for at, o in ((0, off), (1, off), (2, 2), (3, 2), (4, 2), (5, off), (6, 2)):
+            dout, ys, weight, offsets, position, dys, dweight = [P + (o if i == at else 0) for i in range(7)]
+            assert b(dout, dtype, ys, weight, offsets, position, dys, dweight, 4, 2, 8, 16, None) == want, at
+    assert p(None, 0, None, 8, None, P + 2, None, None, None, 0, 0, 2, 8, 16, None) == want
+    assert ffn(offsets=P + 2) == want
+    assert lib.camoe_ex_ffn_bwd(P, P, P, P, P + 1, *[P] * 6, 4, 2, 16, 32, None) == want
+    for adapter, scale in ((P + 2, None), (P, P + 1)):
+        assert lib.camoe_ad_linear(P, P, P, P, adapter, scale, P, P, 1 << 30, 50, 64, 64, 8, 4, None) == want
