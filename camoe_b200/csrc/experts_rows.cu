@@ -9,9 +9,9 @@
 // Up to kSmallSlots slots one launch does it all: each token's block counts its
 // own slots' rows by reading the whole index once (a warp per slot) and copies
 // its row.  Above that every chunk of slots has a block that places them: it adds
-// up the slots of the chunks before it (up to 8192 slots by reading the whole index
-// itself, above from counts per chunk that a first launch makes) and a warp's of
-// the warps before it.  The copy follows; the launches overlap (programmatic
+// up the slots of the chunks before it (up to 8192 slots of few experts by reading
+// the whole index itself, otherwise from counts per chunk that a first launch makes)
+// and a warp's of the warps before it.  The copy follows; the launches overlap (programmatic
 // dependent launches), so that x is loaded by the time the rows are known.
 //
 // The copies are bound by HBM: a thread holds 16 bytes (or one element where the
@@ -169,17 +169,23 @@ inline int64_t chunk_of(int64_t S) {
   const int64_t c = ((S + 255) / 256 + kSortThreads - 1) / kSortThreads * kSortThreads;
   return c > 2 * kSortThreads ? c : 2 * kSortThreads;
 }
-// Whether each block counts all slots itself, one launch less, where its counters fit.
-// Kernel times: 7001 slots 6.0 us, 3.3 + 4.6 in two launches; 16384 slots 10.7 us, 3.1 + 4.3.
-inline bool alone(int64_t S, int64_t E) { return S <= 8192 && E < 512; }
-// Shared memory of place_kernel, and the most that any call asks for: the limit is set
-// to that one, so that host threads with sorts of different sizes do not lower each
-// other's before a launch.
+// Whether each block counts all slots itself, one launch less: dearer on the device
+// (every block reads all slots and sums a counter per warp and expert) and cheaper for
+// the host, which bounds such calls.  us a call in a loop, with the copy of rows of
+// 1024 bf16, so / in two launches, and on the device behind queued work: 2600 slots of 8
+// experts 11.1 / 14.4 (10.3 / 8.3), 8192 of 8 12.4 / 14.5 (12.4 / 10.3), 8192 of 16
+// 14.4 / 14.6 (14.4 / 10.3), 8192 of 24 16.4 / 14.6 (16.4 / 10.3), 8192 of 200 20.5 /
+// 14.4 (20.6 / 12.4).
+constexpr int kAloneExperts = 16;
+inline bool alone(int64_t S, int64_t E) { return S <= 8192 && E <= kAloneExperts; }
+// Shared memory of place_kernel, and the most that any call asks for (alone with few
+// experts asks for little): the limit is set to that one, so that host threads with
+// sorts of different sizes do not lower each other's before a launch.
 constexpr int place_smem(bool solo, int E) {
   return ((solo ? 2 : 1) * kSortWarps + 2) * (E + 1) * static_cast<int>(sizeof(int));
 }
-constexpr int kPlaceSmem = place_smem(false, kMaxExperts) > place_smem(true, 511) ? place_smem(false, kMaxExperts)
-                                                                                  : place_smem(true, 511);
+constexpr int kPlaceSmem = place_smem(false, kMaxExperts);
+static_assert(place_smem(true, kAloneExperts) <= kPlaceSmem, "the most of any call");
 inline int64_t chunks_of(int64_t S) { return (S + chunk_of(S) - 1) / chunk_of(S); }
 
 // slots of each expert in each chunk: counts[chunk][expert]

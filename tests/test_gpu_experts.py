@@ -89,12 +89,12 @@ def test_dispatch_is_the_stable_sort(N, k, E, empty, dtype):
     assert torch.equal(xs, want)
 
 
-@pytest.mark.parametrize("E", [1, 8, 200, 511, 512])
+@pytest.mark.parametrize("E", [1, 8, 16, 17, 200, 511, 512])
 @pytest.mark.parametrize("N,k", [(2049, 1), (2048, 2), (8191, 1), (4096, 2), (2731, 3)])
 def test_dispatch_where_each_block_counts_all_slots(N, k, E):
-    """Up to 8192 slots of fewer than 512 experts are placed in one launch, in which a
-    block counts the slots before its chunk and behind it with the same counters:
-    fresh indices each time, spread, skewed and all of one expert."""
+    """Up to 8192 slots of up to 16 experts are placed in one launch, in which a block
+    counts the slots before its chunk and behind it with the same counters; the others
+    in two.  Fresh indices each time, spread, skewed and all of one expert."""
     x = rnd(N, 8, seed=3)
     for seed in range(4):
         index = index_of(N, k, E, 200 + seed, 0.0 if seed % 2 else 0.2, torch.int32)
