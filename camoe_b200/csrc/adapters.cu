@@ -78,9 +78,12 @@ __global__ void __launch_bounds__(kThreads) low_kernel(const bf16* __restrict__ 
 
 // Rows that are streamed rather than sorted: few, and with little of the adapters' own
 // work, which each row does for itself there.  B200, us streamed / in tiles, rows
-// that mix L adapters, N x C x M x D, L:  128 x 2048 x 2048 x 32, 64: 19 / 53;
-// 256 x 2048 x 2048 x 32, 64: 30 / 58;  384: 49 / 49;  512 x 1024 x 1024 x 16, 12:
-// 23 / 25;  512 x 1024 x 1024 x 64, 3: 51 / 23;  256 x 2048 x 4096 x 128, 64: 132 / 78.
+// that mix L adapters, N x C x M x D, L:  128 x 2048 x 2048 x 32, 64: 19 / 64;
+// 256 x 2048 x 2048 x 32, 64: 31 / 69;  384: 51 / 58;  512 x 1024 x 1024 x 16, 12:
+// 24 / 27;  512 x 1024 x 1024 x 64, 3: 51 / 23;  256 x 2048 x 4096 x 128, 64: 133 / 88.
+// Up to 128 rows all are streamed: 128 x 2048 x 2048 x 128, 64 45 / 82;  64 x 2048 x
+// 4096 x 256, 64 80 / 93;  16: 30 / 56.  The rule is not the best at the highest
+// ranks: 128 x 2048 x 4096 x 256, 64 147 / 112;  128 x 1024 x 1024 x 256, 3 43 / 27.
 bool few_rows(int64_t N, int64_t M, int64_t D) { return N <= 128 || (N <= 512 && N * M * D <= (24 << 20)); }
 
 // A few rows whose low-rank parts are little work for each CTA of a cluster of four

@@ -149,7 +149,8 @@ class ExpertLayer(nn.Module):
     the weighted sum of the chosen experts' outputs in x's dtype.  The products
     run in bf16: fp32 parameters are cast per call, as ``RWKV7TimeMix`` casts
     its own (gradients arrive in fp32); convert the module with ``.bfloat16()``
-    to serve without that."""
+    to serve without that (the same outputs, bit for bit, where bf16 holds the
+    values)."""
 
     def __init__(self, n_embd: int, n_experts: int, hidden: int | None = None):
         super().__init__()

@@ -80,7 +80,10 @@ size_t camoe_ad_work_bytes(int64_t N, int64_t C, int64_t M, int64_t D, int64_t L
  *   y[n] = weight x[n] + scale[a] up[a] (down[a] x[n]),   a = adapter[n]
  * weight [M, C], down [L, D, C], up [L, M, D], scale [L] fp32 (NULL: ones),
  * adapter [N] int32; a row whose adapter is outside [0, L) gets weight x[n]
- * alone.  C, M and D are multiples of 8, D <= 256, L <= 1024. */
+ * alone.  C, M and D are multiples of 8, D <= 256, L <= 1024.  y is rounded once;
+ * with many rows (above 128, or above 512 where N M D <= 24 * 2^20) scale down x is
+ * rounded to bf16 before its product with up.  Values of an adapter that are not
+ * finite reach its own rows only. */
 int camoe_ad_linear(const void* x, const void* weight, const void* down, const void* up,
                     const int32_t* adapter, const float* scale, void* y, void* work,
                     size_t work_bytes, int64_t N, int64_t C, int64_t M, int64_t D, int64_t L,
